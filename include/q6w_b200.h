@@ -345,6 +345,111 @@ Q6W_API int32_t q6w_sample(const float* logits, int64_t ld, int32_t n, int32_t v
                            const q6w_sample_args* sampling, const int32_t* stop_ids, int32_t n_stop,
                            int32_t min_new_tokens, int32_t* tokens, q6w_stream_t stream);
 
+/* ---- serving from a paged cache ------------------------------------------ */
+
+/* One layer of a paged KV cache and one step's batch over it.  No counterpart
+ * in the reference, whose cache is one block per request
+ * (torch_benchmark.py:87-94): here a request holds only the pages its tokens
+ * fill, taken from one pool, and requests may share pages.
+ *
+ * Pools: key (value) element d of kv head g in slot i of page p lies at
+ * k_pages (v_pages) + p*page_stride + i*slot_stride + g*head_stride + d, in
+ * elements of kv_dtype; any strides that are multiples of 16 bytes (a layer
+ * of [layers, pages, page_size, kv_heads, head_dim], pages stored head by
+ * head, K and V side by side).  page_size is a power of two up to 1024,
+ * head_dim 16, 32, 64 or 128.
+ *
+ * Batch: position i of sequence s is slot i % page_size of page
+ * page_table[s*table_stride + i / page_size], for i < lengths[s]; lengths
+ * count the tokens of this step.  With query_starts, tokens
+ * query_starts[s] .. query_starts[s+1]-1 of the step are sequence s's last
+ * ones, in order (any number, also none); NULL: token s is sequence s's last
+ * one.  Table entries at or behind a sequence's last page are not read.
+ *
+ * What the host cannot check is met on the device: a length beyond
+ * max_pages*page_size stands for positions that are not there (never read or
+ * written); a token whose position is negative (more new tokens than the
+ * length) or that no sequence holds (in front of query_starts[0], behind
+ * query_starts[n_seqs]) is padding; a page id outside [0, n_pages) is never
+ * followed.  Such a length and a bad page id set bit 0 of *status (one int32 on the device that the caller zeroes once
+ * and q6w_workspace_status reads; may be NULL). */
+typedef struct q6w_paged_batch {
+  void* k_pages;
+  void* v_pages;
+  int32_t kv_dtype; /* Q6W_KV_F32 or Q6W_KV_F16 */
+  int32_t n_pages, page_size, kv_heads, head_dim;
+  int64_t page_stride, slot_stride, head_stride; /* elements */
+  int32_t n_seqs;
+  int32_t max_pages; /* page-table entries of a sequence */
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* lengths;      /* [n_seqs] */
+  const int32_t* query_starts; /* [n_seqs + 1], or NULL */
+  int32_t* status;
+} q6w_paged_batch;
+
+/* Rotate the step's queries and keys to their positions and append keys and
+ * values to their sequences' pages: the RoPE of torch_benchmark.py:79-85 on
+ * pairs (2j, 2j+1), each product rounded before the add, then the cache write
+ * of :110-112, rounded to nearest even for FP16 pages.  queries
+ * [n_tokens, n_heads, head_dim], keys and values [n_tokens, kv_heads,
+ * head_dim] FP32 with token strides in elements (multiples of 4, so the three
+ * may be parts of one QKV output); rope_cos / rope_sin [rope_len, head_dim/2].
+ * Token positions count from first_position (the length of a shared prefix
+ * in front of the sequence's own pages).  rotated [n_tokens, n_heads,
+ * head_dim] receives the queries (contiguous; it may be queries itself);
+ * queries and rotated are both NULL when n_heads is 0.  Padding tokens write
+ * nothing, neither do positions at or beyond rope_len (which set status
+ * bit 0); their rows of rotated are zeroed when zero_padding is set and left
+ * as they were otherwise.  A bad page id drops the token's key and value.
+ * Two tokens of one call that land in one slot leave either's row. */
+Q6W_API int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
+                                 const float* queries, int64_t query_stride, const float* keys,
+                                 int64_t key_stride, const float* values, int64_t value_stride,
+                                 const float* rope_cos, const float* rope_sin, int32_t rope_len,
+                                 int32_t first_position, float* rotated, int32_t zero_padding,
+                                 q6w_stream_t stream);
+
+/* Workspace bytes of the two attention calls below for n_tokens query tokens
+ * of n_heads heads (prefix_length 0 for q6w_paged_attention); 0 for arguments
+ * that they refuse. */
+Q6W_API size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n_tokens,
+                                         int32_t n_heads, int32_t prefix_length);
+
+/* Causal grouped-query attention of the step's tokens over their sequences'
+ * pages: for the token at position p of sequence s and query head h (kv head
+ * g = h / (n_heads / kv_heads))
+ *   out = sum_{i <= p} softmax_i(q . K[i, g] / sqrt(head_dim)) V[i, g]
+ * -- q6w_gqa_attention for one token a sequence (torch_benchmark.py:113-119),
+ * and a prompt's or a chunk's attention for more.  queries (rotated)
+ * [n_tokens, n_heads, head_dim] FP32 with a token stride in elements
+ * (a multiple of 4); output [n_tokens, n_heads, head_dim] contiguous.
+ * n_heads is a multiple of kv_heads.  Scores, softmax and sums are FP32.  A
+ * token with no visible key (length 0, padding by length) gives zeros; rows
+ * of tokens that no sequence holds are zeroed when zero_padding is set and
+ * left as they were otherwise.  Slots behind a sequence's length may hold anything.  A row that
+ * meets a bad page id is NaN.  workspace: 256-byte aligned,
+ * q6w_paged_workspace_bytes; not read before it is written, so it needs no
+ * clearing and may be shared by calls of one stream. */
+Q6W_API int32_t q6w_paged_attention(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
+                                    const float* queries, int64_t query_stride, float* output,
+                                    int32_t zero_padding, void* workspace, size_t workspace_bytes,
+                                    q6w_stream_t stream);
+
+/* q6w_paged_attention of a batch whose sequences all continue one cached
+ * prefix: every token of the step also sees the prefix_length tokens held in
+ * pages prefix_pages[0 .. ceil(prefix_length / page_size)) (device array) of
+ * the same pools, in front of its sequence's own.  The pool holds the prefix
+ * once and the call reads it once for all tokens.  lengths and page_table
+ * describe the sequences' own tokens only (a length may be 0); own tokens
+ * stand at positions prefix_length + i (q6w_paged_append's first_position).
+ * prefix_length 0 is q6w_paged_attention. */
+Q6W_API int32_t q6w_shared_prefix_attention(const q6w_paged_batch* batch, const int32_t* prefix_pages,
+                                            int32_t prefix_length, int32_t n_tokens, int32_t n_heads,
+                                            const float* queries, int64_t query_stride, float* output,
+                                            int32_t zero_padding, void* workspace,
+                                            size_t workspace_bytes, q6w_stream_t stream);
+
 /* Synchronise `stream` and report device-side errors recorded in the
  * workspace since the last call (then clear them): Q6W_OK, or Q6W_ERR_DEVICE
  * for rejected input (bit 0) or a device wait that ran out of time (bit 2). */

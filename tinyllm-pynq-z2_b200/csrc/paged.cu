@@ -1,0 +1,387 @@
+// Serving from a paged KV cache: append with rotation, causal attention over
+// pages, and attention of a batch behind a shared prefix.
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace q6w {
+namespace paged {
+
+// ---- append ------------------------------------------------------------------
+//
+// One pass: (a, b) -> (a cos - b sin, a sin + b cos) on pairs (2j, 2j+1) of
+// every query and key head at the token's position, the value rows copied.
+// Bound by memory: per token 4 (2 H + 2 KV) head_dim bytes of activations and
+// the page rows.  `tpt` threads take one token (a whole warp at least, so
+// that the search for the token's sequence is a warp's), eight consecutive
+// elements a thread and step: two 16-byte loads, one or two 16-byte stores.
+
+struct AppendArgs {
+  Batch b;
+  const float* q;
+  const float* k;
+  const float* v;
+  int64_t ldq, ldk, ldv;
+  const float* cs;
+  const float* sn;
+  float* out;
+  int32_t hd, H, rope_len, first, zero, tpt_shift;
+};
+
+__device__ __forceinline__ void store8(void* pool, int64_t off, int half, const float (&x)[8]) {
+  if (half) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(static_cast<__half*>(pool) + off) = *reinterpret_cast<const uint4*>(h);
+  } else {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(pool) + off);
+    p[0] = make_float4(x[0], x[1], x[2], x[3]);
+    p[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+template <bool HALF>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int tpt = 1 << a.tpt_shift;
+  const int t = blockIdx.x * (256 >> a.tpt_shift) + (threadIdx.x >> a.tpt_shift);
+  if (t >= a.b.T) return;  // warp-uniform: tpt >= 32
+  const int s = token_seq(a.b, t, lane);
+  int at = -1;  // index among the sequence's own tokens
+  if (s >= 0 && s < a.b.n) {
+    int t0, t1;
+    seq_tokens(a.b, s, t0, t1);
+    at = seq_length(a.b, s) - (t1 - t);
+  }
+  const int64_t pos = (int64_t)a.first + at;
+  if (at < 0 || at >= a.b.max_len || pos >= a.rope_len) {
+    if (at >= 0) flag(a.b.status, kErrInput);
+    if (a.zero)
+      for (int i = threadIdx.x & (tpt - 1); i < a.H * (a.hd >> 2); i += tpt)
+        reinterpret_cast<float4*>(a.out + (int64_t)t * a.H * a.hd)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    return;
+  }
+  const int page = __ldg(a.b.table + s * a.b.table_stride + (at >> a.b.shift));
+  const bool page_ok = page >= 0 && page < a.b.n_pages;
+  if (!page_ok) flag(a.b.status, kErrInput);
+  const int64_t slot = page * a.b.page_stride + (int64_t)(at & ((1 << a.b.shift) - 1)) * a.b.slot_stride;
+  const int hd = a.hd, units = hd >> 3;  // eight-element units of a head
+  const int nq = a.H * units, nk = a.b.kv_heads * units;
+  const float* cs = a.cs + pos * (hd >> 1);
+  const float* sn = a.sn + pos * (hd >> 1);
+  for (int i = threadIdx.x & (tpt - 1); i < nq + 2 * nk; i += tpt) {
+    const float* src;
+    const int j = i < nq ? i : (i < nq + nk ? i - nq : i - nq - nk);
+    if (i < nq)
+      src = a.q + t * a.ldq + 8 * j;
+    else
+      src = (i < nq + nk ? a.k + t * a.ldk : a.v + t * a.ldv) + 8 * j;
+    const float4 lo = __ldcs(reinterpret_cast<const float4*>(src));
+    const float4 hi = __ldcs(reinterpret_cast<const float4*>(src) + 1);
+    float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const int u = j % units;
+    if (i < nq + nk) {
+      const float4 c = __ldg(reinterpret_cast<const float4*>(cs + 4 * u));
+      const float4 d = __ldg(reinterpret_cast<const float4*>(sn + 4 * u));
+      const float cc[4] = {c.x, c.y, c.z, c.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float x0 = x[2 * p], x1 = x[2 * p + 1];
+        x[2 * p] = __fsub_rn(__fmul_rn(x0, cc[p]), __fmul_rn(x1, dd[p]));
+        x[2 * p + 1] = __fadd_rn(__fmul_rn(x0, dd[p]), __fmul_rn(x1, cc[p]));
+      }
+    }
+    if (i < nq) {
+      store8(a.out, ((int64_t)t * a.H) * hd + 8 * j, 0, x);
+    } else if (page_ok) {
+      const int64_t off = slot + (j / units) * a.b.head_stride + 8 * u;
+      store8(i < nq + nk ? a.b.k : a.b.v, off, HALF, x);
+    }
+  }
+}
+
+// ---- attention -----------------------------------------------------------------
+
+struct AttnArgs {
+  Batch b;
+  const float* q;
+  int64_t ldq;
+  float* out;
+  int32_t H, zero;
+  const int32_t* prefix_pages;
+  int32_t prefix_len;
+  float scale;  // log2(e) / sqrt(head_dim)
+};
+
+template <int HD>
+__device__ __forceinline__ float key_dot(const float* q, const float* k) {
+  float d = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD; i += 4) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(k + i));
+    d = fmaf(q[i], x.x, d);
+    d = fmaf(q[i + 1], x.y, d);
+    d = fmaf(q[i + 2], x.z, d);
+    d = fmaf(q[i + 3], x.w, d);
+  }
+  return d;
+}
+template <int HD>
+__device__ __forceinline__ float key_dot(const float* q, const __half* k) {
+  float d = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD; i += 2) {
+    const float2 x = __half22float2(__ldg(reinterpret_cast<const __half2*>(k + i)));
+    d = fmaf(q[i], x.x, d);
+    d = fmaf(q[i + 1], x.y, d);
+  }
+  return d;
+}
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+
+// One warp per (token, query head); a lane takes every 32nd visible key with
+// a running maximum and sum of its own, the lanes' states joined at the end.
+template <int HD, typename KT>
+__global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
+  __shared__ float qs[4][HD];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = (int64_t)blockIdx.x * 4 + warp;
+  if (item >= (int64_t)a.b.T * a.H) return;
+  const int t = (int)(item / a.H), h = (int)(item % a.H), g = h / a.b.rep;
+  float* out = a.out + item * HD;
+  const int s = token_seq(a.b, t, lane);
+  if (s < 0 || s >= a.b.n) {
+    if (a.zero)
+      for (int d = lane; d < HD; d += 32) out[d] = 0.f;
+    return;
+  }
+  for (int d = lane; d < HD; d += 32) qs[warp][d] = a.q[t * a.ldq + h * HD + d];
+  __syncwarp();
+  int t0, t1;
+  seq_tokens(a.b, s, t0, t1);
+  const int seen = min(max(seq_length(a.b, s) - (t1 - t) + 1, 0), a.b.max_len);
+  float m = -INFINITY, l = 0.f, acc[HD];
+#pragma unroll
+  for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+  const int P = a.prefix_len;
+  for (int64_t i = lane; i < (int64_t)P + seen; i += 32) {
+    const int at = (int)(i < P ? i : i - P);
+    const int32_t* ids = i < P ? a.prefix_pages : a.b.table + s * a.b.table_stride;
+    const int page = __ldg(ids + (at >> a.b.shift));
+    float sc;
+    const KT* vr = nullptr;
+    if (page < 0 || page >= a.b.n_pages) {
+      flag(a.b.status, kErrInput);
+      sc = NAN;
+    } else {
+      const int64_t off = page * a.b.page_stride + (int64_t)(at & ((1 << a.b.shift) - 1)) * a.b.slot_stride +
+                          g * a.b.head_stride;
+      sc = key_dot<HD>(qs[warp], static_cast<const KT*>(a.b.k) + off) * a.scale;
+      vr = static_cast<const KT*>(a.b.v) + off;
+    }
+    const float mn = fmaxf(m, sc);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float al = exp2f(m - ref), p = exp2f(sc - ref);
+    m = mn;
+    l = l * al + p;
+#pragma unroll
+    for (int d = 0; d < HD; ++d) acc[d] = fmaf(p, vr ? widen(vr[d]) : 0.f, acc[d] * al);
+  }
+  float M = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = M == -INFINITY ? 0.f : M;
+  const float w = exp2f(m - ref);
+  float L = l * w;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+  for (int d = 0; d < HD; ++d) {
+    float x = acc[d] * w;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == (d & 31)) out[d] = L == 0.f ? 0.f : x / L;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+
+static int32_t check_batch(const char* who, const q6w_paged_batch* p, int32_t n_tokens, Batch* b) {
+  if (!p) return fail(Q6W_ERR_ARG, "%s: null batch", who);
+  if (p->kv_dtype != Q6W_KV_F32 && p->kv_dtype != Q6W_KV_F16) return fail(Q6W_ERR_ARG, "%s: unknown kv_dtype", who);
+  const int hd = p->head_dim;
+  if (hd != 16 && hd != 32 && hd != 64 && hd != 128)
+    return fail(Q6W_ERR_ARG, "%s: head_dim %d unsupported (16, 32, 64 or 128)", who, hd);
+  if (p->page_size < 1 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+    return fail(Q6W_ERR_ARG, "%s: page_size %d is not a power of two up to 1024", who, p->page_size);
+  if (p->kv_heads < 1 || p->kv_heads > 1024 || p->n_pages < 0 || p->n_seqs < 0 || p->max_pages < 0 || n_tokens < 0)
+    return fail(Q6W_ERR_ARG, "%s: bad shape", who);
+  if ((int64_t)p->max_pages * p->page_size > (1 << 30))
+    return fail(Q6W_ERR_ARG, "%s: a sequence of up to %lld tokens is too long", who,
+                (long long)p->max_pages * p->page_size);
+  if (n_tokens > (1 << 24) || p->n_seqs > (1 << 24)) return fail(Q6W_ERR_ARG, "%s: more than 2^24 tokens", who);
+  if (!p->query_starts && n_tokens != p->n_seqs)
+    return fail(Q6W_ERR_ARG, "%s: %d tokens for %d sequences need query_starts", who, n_tokens, p->n_seqs);
+  const int64_t unit = p->kv_dtype == Q6W_KV_F16 ? 8 : 4;  // elements of 16 bytes
+  if (p->page_stride % unit || p->slot_stride % unit || p->head_stride % unit || p->page_stride < 0 ||
+      p->slot_stride < 0 || p->head_stride < 0)
+    return fail(Q6W_ERR_ALIGN, "%s: page, slot and head strides must be multiples of 16 bytes", who);
+  if (n_tokens > 0 && p->n_seqs > 0) {
+    if (!p->k_pages || !p->v_pages || !p->lengths || (p->max_pages > 0 && !p->page_table))
+      return fail(Q6W_ERR_ARG, "%s: null pointer", who);
+    if (!aligned(p->k_pages, 16) || !aligned(p->v_pages, 16))
+      return fail(Q6W_ERR_ALIGN, "%s: pages must be 16-byte aligned", who);
+  }
+  b->k = p->k_pages;
+  b->v = p->v_pages;
+  b->page_stride = p->page_stride;
+  b->slot_stride = p->slot_stride;
+  b->head_stride = p->head_stride;
+  b->table = p->page_table;
+  b->table_stride = p->table_stride;
+  b->lengths = p->lengths;
+  b->starts = p->query_starts;
+  b->status = p->status;
+  b->n = p->n_seqs;
+  b->T = n_tokens;
+  b->n_pages = p->n_pages;
+  b->shift = __builtin_ctz((unsigned)p->page_size);
+  b->max_len = p->max_pages * p->page_size;
+  b->kv_heads = p->kv_heads;
+  b->rep = 1;
+  return Q6W_OK;
+}
+
+static int32_t check_heads(const char* who, const q6w_paged_batch* p, int32_t n_heads, Batch* b) {
+  if (n_heads < 1 || n_heads > (1 << 14) || n_heads % p->kv_heads)
+    return fail(Q6W_ERR_ARG, "%s: %d query heads are not a multiple of %d kv heads", who, n_heads, p->kv_heads);
+  b->rep = n_heads / p->kv_heads;
+  return Q6W_OK;
+}
+
+template <int HD>
+static void launch_rows(const AttnArgs& a, bool half, cudaStream_t st) {
+  const unsigned grid = (unsigned)(((int64_t)a.b.T * a.H + 3) / 4);
+  if (half)
+    attn_rows_kernel<HD, __half><<<grid, 128, 0, st>>>(a);
+  else
+    attn_rows_kernel<HD, float><<<grid, 128, 0, st>>>(a);
+}
+
+static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_t* prefix_pages, int32_t prefix_length,
+                         int32_t n_tokens, int32_t n_heads, const float* queries, int64_t query_stride, float* output,
+                         int32_t zero_padding, void* workspace, size_t workspace_bytes, q6w_stream_t stream) {
+  clear_error();
+  AttnArgs a;
+  int32_t st = check_batch(who, p, n_tokens, &a.b);
+  if (st) return st;
+  st = check_heads(who, p, n_heads, &a.b);
+  if (st) return st;
+  if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
+  if (n_tokens == 0) return Q6W_OK;
+  if (!queries || !output || (prefix_length > 0 && !prefix_pages)) return fail(Q6W_ERR_ARG, "%s: null pointer", who);
+  if (!aligned(queries, 16) || !aligned(output, 16) || query_stride % 4)
+    return fail(Q6W_ERR_ALIGN, "%s: queries (and their stride) and output must be 16-byte aligned", who);
+  if (query_stride < (int64_t)n_heads * p->head_dim)
+    return fail(Q6W_ERR_ARG, "%s: query_stride is shorter than a token's heads", who);
+  const size_t need = q6w_paged_workspace_bytes(p, n_tokens, n_heads, prefix_length);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(Q6W_ERR_ARG, "%s: the workspace needs %zu bytes", who, need);
+  a.q = queries;
+  a.ldq = query_stride;
+  a.out = output;
+  a.H = n_heads;
+  a.zero = zero_padding;
+  a.prefix_pages = prefix_pages;
+  a.prefix_len = prefix_length;
+  a.scale = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
+  const bool half = p->kv_dtype == Q6W_KV_F16;
+  cudaStream_t s = (cudaStream_t)stream;
+  switch (p->head_dim) {
+    case 16: launch_rows<16>(a, half, s); break;
+    case 32: launch_rows<32>(a, half, s); break;
+    case 64: launch_rows<64>(a, half, s); break;
+    default: launch_rows<128>(a, half, s); break;
+  }
+  Q6W_LAUNCH_CHECK("attn_rows_kernel");
+  return Q6W_OK;
+}
+
+}  // namespace paged
+}  // namespace q6w
+
+using namespace q6w;
+
+extern "C" int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
+                                    const float* queries, int64_t query_stride, const float* keys,
+                                    int64_t key_stride, const float* values, int64_t value_stride,
+                                    const float* rope_cos, const float* rope_sin, int32_t rope_len,
+                                    int32_t first_position, float* rotated, int32_t zero_padding,
+                                    q6w_stream_t stream) {
+  const char* who = "q6w_paged_append";
+  clear_error();
+  paged::AppendArgs a;
+  int32_t st = paged::check_batch(who, batch, n_tokens, &a.b);
+  if (st) return st;
+  if (n_heads < 0 || n_heads > (1 << 14)) return fail(Q6W_ERR_ARG, "%s: bad n_heads", who);
+  if (rope_len < 0 || first_position < 0) return fail(Q6W_ERR_ARG, "%s: negative rope_len or first_position", who);
+  if (n_tokens == 0) return Q6W_OK;
+  if (!keys || !values || !rope_cos || !rope_sin || (n_heads > 0 && (!queries || !rotated)))
+    return fail(Q6W_ERR_ARG, "%s: null pointer", who);
+  if (!aligned(keys, 16) || !aligned(values, 16) || !aligned(queries, 16) || !aligned(rotated, 16) ||
+      !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || query_stride % 4 || key_stride % 4 || value_stride % 4)
+    return fail(Q6W_ERR_ALIGN, "%s: tensors and token strides must be 16-byte aligned", who);
+  const int64_t kv_row = (int64_t)batch->kv_heads * batch->head_dim;
+  if (key_stride < kv_row || value_stride < kv_row || (n_heads > 0 && query_stride < (int64_t)n_heads * batch->head_dim))
+    return fail(Q6W_ERR_ARG, "%s: a token stride is shorter than a token's heads", who);
+  if (rotated == queries && n_heads > 0 && query_stride != (int64_t)n_heads * batch->head_dim)
+    return fail(Q6W_ERR_ARG, "%s: queries rotated in place must be contiguous", who);
+  a.q = queries;
+  a.k = keys;
+  a.v = values;
+  a.ldq = query_stride;
+  a.ldk = key_stride;
+  a.ldv = value_stride;
+  a.cs = rope_cos;
+  a.sn = rope_sin;
+  a.out = rotated;
+  a.hd = batch->head_dim;
+  a.H = n_heads;
+  a.rope_len = rope_len;
+  a.first = first_position;
+  a.zero = zero_padding;
+  const int units = (n_heads + 2 * batch->kv_heads) * (batch->head_dim >> 3);
+  a.tpt_shift = 5;
+  while (a.tpt_shift < 8 && (1 << a.tpt_shift) < units) ++a.tpt_shift;
+  const int per = 256 >> a.tpt_shift;
+  const unsigned grid = (unsigned)((n_tokens + per - 1) / per);
+  if (batch->kv_dtype == Q6W_KV_F16)
+    paged::append_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+  else
+    paged::append_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+  Q6W_LAUNCH_CHECK("append_kernel");
+  return Q6W_OK;
+}
+
+extern "C" size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
+                                            int32_t prefix_length) {
+  return 0;
+}
+
+extern "C" int32_t q6w_paged_attention(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
+                                       const float* queries, int64_t query_stride, float* output, int32_t zero_padding,
+                                       void* workspace, size_t workspace_bytes, q6w_stream_t stream) {
+  return paged::attention("q6w_paged_attention", batch, nullptr, 0, n_tokens, n_heads, queries, query_stride, output,
+                          zero_padding, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t q6w_shared_prefix_attention(const q6w_paged_batch* batch, const int32_t* prefix_pages,
+                                               int32_t prefix_length, int32_t n_tokens, int32_t n_heads,
+                                               const float* queries, int64_t query_stride, float* output,
+                                               int32_t zero_padding, void* workspace, size_t workspace_bytes,
+                                               q6w_stream_t stream) {
+  return paged::attention("q6w_shared_prefix_attention", batch, prefix_pages, prefix_length, n_tokens, n_heads, queries,
+                          query_stride, output, zero_padding, workspace, workspace_bytes, stream);
+}

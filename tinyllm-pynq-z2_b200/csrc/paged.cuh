@@ -1,0 +1,77 @@
+// Paged KV cache: what the append and attention kernels share.
+//
+// A sequence's cache is a list of page ids (a row of the page table) into one
+// pool; position i is slot i % page_size of page i / page_size.  One key (or
+// value) of one kv head is head_dim contiguous elements; pages, slots and kv
+// heads have strides of their own.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "async.cuh"
+#include "common.cuh"
+
+namespace q6w {
+namespace paged {
+
+constexpr int32_t kErrInput = 1;    // status bit 0: rejected input (a length, a page id, a position)
+constexpr int32_t kErrTimeout = 4;  // status bit 2: a bounded wait ran out
+
+struct Batch {
+  void* k;
+  void* v;
+  int64_t page_stride, slot_stride, head_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int32_t* status;
+  int32_t n, T, n_pages, shift, max_len, kv_heads, rep;
+};
+
+__device__ __forceinline__ void flag(int32_t* status, int32_t bit) {
+  if (status) atomicOr(status, bit);
+}
+
+// Tokens that sequence s claims (the step's own included), never negative.  A
+// length that its page-table row cannot hold is flagged; positions from
+// max_len on do not exist.
+__device__ __forceinline__ int seq_length(const Batch& b, int s) {
+  const int len = __ldg(b.lengths + s);
+  if (len > b.max_len) flag(b.status, kErrInput);
+  return max(len, 0);
+}
+
+// First and one-past-last query token of sequence s, kept inside [0, T].
+__device__ __forceinline__ void seq_tokens(const Batch& b, int s, int& t0, int& t1) {
+  if (!b.starts) {
+    t0 = s;
+    t1 = s + 1;
+    return;
+  }
+  t0 = min(max(__ldg(b.starts + s), 0), b.T);
+  t1 = min(max(__ldg(b.starts + s + 1), t0), b.T);
+}
+
+// Sequence of query token t, by the whole warp (all lanes the same t): the
+// last s with starts[s] <= t, found 32-fold a round.  -1 or n: no sequence.
+__device__ __forceinline__ int token_seq(const Batch& b, int t, int lane) {
+  if (!b.starts) return t;
+  int lo = 0, hi = b.n + 1;  // starts[i] <= t for i < lo; starts[i] > t for i >= hi
+  while (lo < hi) {
+    const int step = (hi - lo + 31) >> 5;
+    const int i = lo + lane * step;
+    const bool le = i < hi && __ldg(b.starts + i) <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, le));
+    if (c == 0) {
+      hi = lo;
+    } else {
+      hi = min(hi, lo + c * step);
+      lo += (c - 1) * step + 1;
+    }
+  }
+  return lo - 1;
+}
+
+}  // namespace paged
+}  // namespace q6w

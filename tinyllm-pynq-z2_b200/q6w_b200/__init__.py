@@ -26,7 +26,8 @@ def __getattr__(name):
 
         return getattr(model, name)
     if name in ("unpack_signed_int6", "dequantize_rows", "q6w_linear", "load_dequantized_state", "DeviceImage",
-                "linear_argmax", "rmsnorm", "gqa_attention"):
+                "linear_argmax", "rmsnorm", "gqa_attention", "paged_append", "paged_attention",
+                "shared_prefix_attention", "check_status"):
         from . import ops
 
         return getattr(ops, name)

@@ -28,6 +28,7 @@ EXPORTS = (
     "q6w_rmsnorm", "q6w_gqa_attention", "q6w_linear_argmax_noalloc", "q6w_prefill_workspace_bytes",
     "q6w_prefill", "q6w_quantize_rows", "q6w_linear_workspace_bytes", "q6w_linear_ex", "q6w_generate",
     "q6w_sample", "q6w_model_set_kv_dtype", "q6w_forward_all", "q6w_selftest_wait_timeout",
+    "q6w_paged_append", "q6w_paged_workspace_bytes", "q6w_paged_attention", "q6w_shared_prefix_attention",
 )
 
 
@@ -74,6 +75,14 @@ class GreedyArgs(ctypes.Structure):
                 ("step_logits", c_void_p), ("prefill_event", c_void_p)]
 
 
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("kv_dtype", c_int32), ("n_pages", c_int32),
+                ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_stride", c_int64),
+                ("slot_stride", c_int64), ("head_stride", c_int64), ("n_seqs", c_int32), ("max_pages", c_int32),
+                ("page_table", c_void_p), ("table_stride", c_int64), ("lengths", c_void_p),
+                ("query_starts", c_void_p), ("status", c_void_p)]
+
+
 _lib = None
 _load_error = None
 
@@ -113,6 +122,13 @@ def _declare(lib):
                                       c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, S]),
         "q6w_prefill": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int64, c_void_p,
                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t, S]),
+        "q6w_paged_append": (c_int32, [POINTER(PagedBatch), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64,
+                                       c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, S]),
+        "q6w_paged_workspace_bytes": (c_size_t, [POINTER(PagedBatch), c_int32, c_int32, c_int32]),
+        "q6w_paged_attention": (c_int32, [POINTER(PagedBatch), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int32,
+                                          c_void_p, c_size_t, S]),
+        "q6w_shared_prefix_attention": (c_int32, [POINTER(PagedBatch), c_void_p, c_int32, c_int32, c_int32, c_void_p,
+                                                  c_int64, c_void_p, c_int32, c_void_p, c_size_t, S]),
         "q6w_gqa_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int64, S]),
     }

@@ -268,3 +268,179 @@ def gqa_attention(queries, keys, values, lengths, groups_per_kv):
                                          lengths.to(torch.int32).contiguous().data_ptr(), n, kv, groups_per_kv, hd,
                                          max_len, keys.stride(0), _lib.stream_handle()), "q6w_gqa_attention")
     return out
+
+
+# ---- serving from a paged cache -------------------------------------------------
+
+_KV_DTYPES = {torch.float32: 0, torch.float16: 1}
+
+
+def _int32(name, t, device, dim):
+    if t.dtype != torch.int32 or t.device != device or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor of {dim} dimension(s) on {device} with contiguous rows")
+    return t.data_ptr()
+
+
+def _token_rows(name, t, heads, hd, device):
+    """Token stride of t [T, heads, hd] FP32: heads contiguous, tokens at any stride."""
+    if t.dtype != torch.float32 or t.device != device or t.dim() != 3 or t.shape[2] != hd or (
+            heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be float32 [tokens, heads, {hd}] on {device}")
+    T, H, _ = t.shape
+    st = t.stride()
+    if t.numel() and (st[2] != 1 or (H > 1 and st[1] != hd)):
+        raise ValueError(f"the heads of a token of {name} must be contiguous")
+    return st[0] if T > 1 else H * hd
+
+
+def _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, n_tokens):
+    device = key_pages.device
+    if device.type != "cuda":
+        raise ValueError("q6w_b200 ops run on CUDA devices only")
+    kv = _KV_DTYPES.get(key_pages.dtype)
+    if kv is None or value_pages.dtype != key_pages.dtype or value_pages.device != device:
+        raise ValueError("key_pages and value_pages must both be float32 or float16 on one device")
+    if key_pages.dim() != 4 or value_pages.shape != key_pages.shape or value_pages.stride() != key_pages.stride():
+        raise ValueError("key_pages and value_pages must be [pages, page_size, kv_heads, head_dim] with equal strides")
+    pages, page_size, kv_heads, hd = key_pages.shape
+    sp, ss, sh, sd = key_pages.stride()
+    if sd != 1:
+        raise ValueError("the last dimension of the pages must be contiguous")
+    table = _int32("page_table", page_table, device, 2)
+    n, width = page_table.shape
+    lens = _int32("lengths", lengths, device, 1)
+    if lengths.shape[0] != n:
+        raise ValueError(f"lengths must have one entry for each of the {n} rows of page_table")
+    starts = None
+    if query_starts is not None:
+        starts = _int32("query_starts", query_starts, device, 1)
+        if query_starts.shape[0] != n + 1:
+            raise ValueError(f"query_starts must have {n + 1} entries")
+    elif n_tokens != n:
+        raise ValueError(f"{n_tokens} tokens of {n} sequences need query_starts")
+    flags = None if status is None else _int32("status", status, device, 1)
+    if status is not None and status.shape[0] < 1:
+        raise ValueError("status must have an entry")
+    return _lib.PagedBatch(key_pages.data_ptr(), value_pages.data_ptr(), kv, pages, page_size, kv_heads, hd, sp, ss, sh,
+                           n, width, table, page_table.stride(0), lens, starts, flags)
+
+
+def _on_device(device):
+    """Make ``device`` current for a call; nothing to do when it is."""
+    import contextlib
+
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def paged_append(queries, keys, values, cos, sin, key_pages, value_pages, page_table, lengths, query_starts=None,
+                 first_position=0, status=None, out=None):
+    """Rotate a step's queries and keys (RoPE) and append its keys and values
+    to the pages of their sequences, in one pass.
+
+    queries [T, heads, hd] (or None), keys and values [T, kv_heads, hd]
+    float32, tokens at any stride (parts of one QKV output, say); cos and sin
+    [positions, hd / 2] (``Q6WCudaTransformer.freqs_cos`` / ``freqs_sin``).
+    key_pages and value_pages [pages, page_size, kv_heads, hd] float32 or
+    float16, page_size a power of two; page_table int32 [n, max_pages];
+    lengths int32 [n], each sequence's tokens including this step's;
+    query_starts int32 [n + 1], the step's tokens of every sequence (None:
+    one token each).  ``first_position`` is added to a token's position for
+    the rotation (the length of a shared prefix).  Returns the rotated
+    queries, in ``out`` if given (which may be ``queries``); tokens that no
+    sequence holds append nothing, their rows come back zero (in ``out``: as
+    they were).
+
+    ``status``: int32 [1] on the device, zeroed once; bit 0 is set when a
+    length, page id or position is out of range (``check_status``).
+    """
+    device = key_pages.device
+    T = keys.shape[0]
+    b = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
+    kv_heads, hd = b.kv_heads, b.head_dim
+    ldk = _token_rows("keys", keys, kv_heads, hd, device)
+    ldv = _token_rows("values", values, kv_heads, hd, device)
+    if values.shape[0] != T or (queries is not None and queries.shape[0] != T):
+        raise ValueError("queries, keys and values must have the same number of tokens")
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.device != device or t.dim() != 2 or t.shape[1] * 2 != hd or not t.is_contiguous():
+            raise ValueError(f"cos and sin must be contiguous float32 [positions, {hd // 2}] on {device}")
+    if cos.shape != sin.shape:
+        raise ValueError("cos and sin must have the same shape")
+    H = ldq = 0
+    q = rot = None
+    zero = out is None
+    if queries is not None:
+        ldq = _token_rows("queries", queries, None, hd, device)
+        H = queries.shape[1]
+        if zero:
+            out = torch.empty((T, H, hd), dtype=torch.float32, device=device)
+        elif out.shape != queries.shape or out.dtype != torch.float32 or out.device != device or not out.is_contiguous():
+            raise ValueError("out must be contiguous float32 of the queries' shape")
+        q, rot = queries.data_ptr(), out.data_ptr()
+    lib = _lib.load()
+    with _on_device(device):
+        _lib.check(lib.q6w_paged_append(b, T, H, q, ldq, keys.data_ptr(), ldk, values.data_ptr(), ldv, cos.data_ptr(),
+                                        sin.data_ptr(), cos.shape[0], int(first_position), rot, zero,
+                                        _lib.stream_handle()), "q6w_paged_append")
+    return out if queries is not None else None
+
+
+def paged_attention(queries, key_pages, value_pages, page_table, lengths, query_starts=None, status=None, out=None):
+    """Causal grouped-query attention of a step's tokens over paged caches:
+    ``gqa_attention`` for one token a sequence, and the attention of prompts
+    or chunks of prompts for more (``query_starts``).
+
+    queries [T, heads, hd] float32 (rotated; tokens at any stride), the
+    other arguments as ``paged_append`` takes them, after it has run: a token
+    sees its sequence's positions up to its own.  Returns [T, heads, hd];
+    a token without a visible key gives zeros, and so do rows of tokens that
+    no sequence holds (in ``out``, if given, they stay as they were).
+    """
+    return _paged_attention(queries, key_pages, value_pages, None, 0, page_table, lengths, query_starts, status, out)
+
+
+def shared_prefix_attention(queries, key_pages, value_pages, prefix_pages, prefix_length, page_table, lengths,
+                            query_starts=None, status=None, out=None):
+    """``paged_attention`` of a batch whose sequences all continue one prefix:
+    every token also sees the ``prefix_length`` tokens in pages
+    ``prefix_pages`` (int32, on the device) of the same pool, which are read
+    once for the whole batch.  page_table and lengths describe the sequences'
+    own tokens (a length may be 0); their positions start at prefix_length
+    (``paged_append(..., first_position=prefix_length)``).
+    """
+    pages = _int32("prefix_pages", prefix_pages, key_pages.device, 1)
+    if prefix_length < 0 or prefix_length > prefix_pages.shape[0] * key_pages.shape[1]:
+        raise ValueError("prefix_length is more than prefix_pages hold")
+    return _paged_attention(queries, key_pages, value_pages, pages, int(prefix_length), page_table, lengths,
+                            query_starts, status, out)
+
+
+def _paged_attention(queries, key_pages, value_pages, prefix_pages, prefix_length, page_table, lengths, query_starts,
+                     status, out):
+    device = key_pages.device
+    T, H = queries.shape[:2]
+    b = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
+    hd = b.head_dim
+    ldq = _token_rows("queries", queries, None, hd, device)
+    zero = out is None
+    if zero:
+        out = torch.empty((T, H, hd), dtype=torch.float32, device=device)
+    elif out.shape != queries.shape or out.dtype != torch.float32 or out.device != device or not out.is_contiguous():
+        raise ValueError("out must be contiguous float32 of the queries' shape")
+    lib = _lib.load()
+    with _on_device(device):
+        need = lib.q6w_paged_workspace_bytes(b, T, H, prefix_length)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _lib.check(lib.q6w_shared_prefix_attention(b, prefix_pages, prefix_length, T, H, queries.data_ptr(), ldq,
+                                                   out.data_ptr(), zero, ws.data_ptr() if need else None, need,
+                                                   _lib.stream_handle()), "paged attention")
+    return out
+
+
+def check_status(status):
+    """Synchronise and raise Q6WError if a paged call set ``status`` (then clear it)."""
+    lib = _lib.load()
+    with _on_device(status.device):
+        _lib.check(lib.q6w_workspace_status(status.data_ptr(), _lib.stream_handle()), "paged cache")
