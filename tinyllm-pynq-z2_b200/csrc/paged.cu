@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "paged.cuh"
+#include "paged_decode.cuh"
 
 namespace q6w {
 namespace paged {
@@ -299,6 +300,20 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
   a.scale = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
   const bool half = p->kv_dtype == Q6W_KV_F16;
   cudaStream_t s = (cudaStream_t)stream;
+  if (!p->query_starts && prefix_length == 0) {
+    DecodeArgs d;
+    d.b = a.b;
+    d.q = queries;
+    d.ldq = query_stride;
+    d.out = output;
+    d.H = n_heads;
+    d.HB = (a.b.rep + 7) / 8;
+    d.per = (a.b.rep + d.HB - 1) / d.HB;
+    d.scale = a.scale;
+    d.desc = static_cast<int4*>(workspace);
+    d.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)sm_count() * 64);
+    return decode_attention(d, p->head_dim, half, s);
+  }
   switch (p->head_dim) {
     case 16: launch_rows<16>(a, half, s); break;
     case 32: launch_rows<32>(a, half, s); break;
@@ -367,7 +382,11 @@ extern "C" int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_toke
 
 extern "C" size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
                                             int32_t prefix_length) {
-  return 0;
+  paged::Batch b;
+  if (paged::check_batch("q6w_paged_workspace_bytes", batch, n_tokens, &b) ||
+      paged::check_heads("q6w_paged_workspace_bytes", batch, n_heads, &b) || prefix_length < 0)
+    return 0;
+  return batch->query_starts || prefix_length ? 0 : paged::decode_workspace(batch->head_dim);
 }
 
 extern "C" int32_t q6w_paged_attention(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
