@@ -18,7 +18,7 @@ template <int HD, typename KT, int R>
 static int32_t launch(DecodeArgs a, cudaStream_t st) {
   using S = DecodeShape<HD, KT, R>;
   auto kern = decode_kernel<HD, KT, R>;
-  constexpr int smem = 2 * kDecodeWarps * S::STATE * (int)sizeof(float);
+  constexpr int smem = kDecodeWarps * S::WARP;
   // per device: CTAs an SM, with the kernel's shared memory granted once
   static std::mutex mu;
   static int per_sm[64] = {0};

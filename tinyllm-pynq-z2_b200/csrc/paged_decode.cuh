@@ -42,7 +42,9 @@ struct DecodeShape {
   static constexpr int EPL = 16 / (int)sizeof(KT);  // elements of a key that a lane holds
   static constexpr int L = HD / EPL;                // lanes of a key
   static constexpr int G = 32 / L;                  // keys side by side
-  static constexpr int U = (R * EPL >= 64) ? 2 : 4; // steps in flight
+  static constexpr int U = R * EPL > 16 ? 2 : 4;    // steps of an iteration
+  static constexpr int CTAS = R * EPL > 32 ? 1 : 2; // CTAs an SM: 64 + 64 registers of q and o leave room for one
+  static constexpr int STG = CTAS == 1 ? 8 : (U == 4 ? 3 : 4);  // iterations in the ring: 8 to 16 KB a warp
   static constexpr int KPI = G * U;                 // keys of an iteration
   static constexpr int CH = KPI > 16 ? KPI : 16;    // keys of a unit
   static constexpr int NV = U * R;
@@ -50,6 +52,10 @@ struct DecodeShape {
   static constexpr int DUP = NV < L ? L / NV : 1;   // lanes that own the same score
   static constexpr int RL = NS < R ? NS : R;        // query heads among them
   static constexpr int STATE = state_floats(HD, R);
+  // a warp's shared memory: the state of its first piece, the ring (and in it, once
+  // it has been consumed, the state of its last piece)
+  static constexpr int RING = STG * U * 2 * 512;
+  static constexpr int WARP = STATE * 4 + (RING > STATE * 4 ? RING : STATE * 4);
 };
 
 struct DecodeArgs {
@@ -165,13 +171,50 @@ struct Seg {
   int s, block, valid, begin, end;
 };
 
+// A warp's place on the line: the piece [u0, u1) of an item.
+template <int CH>
+struct Cursor {
+  int64_t x, x1, first;
+  int s, block, keys, us, u0, u1, key0, key1;
+  __device__ __forceinline__ void piece() {
+    u1 = (int)min((int64_t)us, u0 + (x1 - x));
+    key0 = u0 * CH;
+    key1 = min(u1 * CH, keys);
+  }
+  __device__ __forceinline__ void next(const Batch& b, int KVB) {
+    x += u1 - u0;
+    u0 = 0;
+    if (u1 == us && ++block == KVB) {
+      block = 0;
+      first += us;
+      ++s;
+      if (x < x1) {
+        keys = keys_of(b, s);
+        us = units_of<CH>(keys);
+      }
+    }
+    piece();
+  }
+};
+
+// 16 bytes from global to shared memory, or 16 zero bytes.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <int HD, typename KT, int R>
-__global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HD, KT, R>::CTAS) decode_kernel(DecodeArgs a) {
   using S = DecodeShape<HD, KT, R>;
   constexpr int EPL = S::EPL, L = S::L, G = S::G, U = S::U, NS = S::NS, RL = S::RL, DUP = S::DUP, CH = S::CH;
   constexpr int E2 = EPL / 2;
   constexpr unsigned kAll = 0xffffffffu;
-  extern __shared__ float slots[];  // [warp][2][STATE]
+  constexpr int STG = S::STG;
+  extern __shared__ __align__(16) uint8_t smem[];  // [warp][WARP]
   __shared__ Line line;
   __shared__ Seg segs[2 * kDecodeWarps];
   const Batch& b = a.b;
@@ -186,18 +229,78 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
   const int64_t wi = (int64_t)blockIdx.x * aw + warp;
   const bool active = warp < aw && wi < workers;
   if (lane < 2) segs[2 * warp + lane].valid = 0;
+  uint8_t* mine = smem + warp * S::WARP;
   if (active) {
-    int64_t x = wi * units / workers;
-    const int64_t x1 = (wi + 1) * units / workers, xb = x;
-    int s;
-    int64_t first;
-    find_seq<CH>(b, line, x / KVB, lane, s, first);
-    int keys = keys_of(b, s), us = units_of<CH>(keys);
-    int block = (int)((x - first * KVB) / us);
-    int u0 = (int)((x - first * KVB) % us);
-    while (x < x1) {
-      const int u1 = (int)min((int64_t)us, u0 + (x1 - x));
-      const int key0 = u0 * CH, key1 = min(u1 * CH, keys);
+    Cursor<CH> c;
+    c.x = wi * units / workers;
+    c.x1 = (wi + 1) * units / workers;
+    const int64_t xb = c.x;
+    find_seq<CH>(b, line, c.x / KVB, lane, c.s, c.first);
+    c.keys = keys_of(b, c.s);
+    c.us = units_of<CH>(c.keys);
+    c.block = (int)((c.x - c.first * KVB) / c.us);
+    c.u0 = (int)((c.x - c.first * KVB) % c.us);
+    c.piece();
+    // The loads run STG - 1 iterations ahead of the arithmetic, over the ends
+    // of items, into a ring that is private to each lane (a lane reads the 16
+    // bytes that it copied itself, so waiting for its own copies is enough).
+    const uint32_t ring = smem_u32(mine) + S::STATE * 4 + lane * 16;
+    const uint4* ring_g = reinterpret_cast<const uint4*>(mine + S::STATE * 4) + lane;
+    Cursor<CH> p = c;
+    const KT* kb = static_cast<const KT*>(b.k) + li * EPL;
+    const KT* vb = static_cast<const KT*>(b.v) + li * EPL;
+    const int32_t* row = b.table;
+    int pt = 0, pbase = 0, plast = -1, ids = -1;  // page ids: lane i holds the id of page pbase + i
+    int64_t hoff = 0;
+    uint32_t bad = 0;  // bit stage * U + u: the key's page id is out of range
+    auto enter = [&]() {  // the first piece from p on that has keys
+      while (p.x < p.x1 && p.key0 >= p.key1) p.next(b, KVB);
+      if (p.x >= p.x1) return;
+      pt = p.key0;
+      row = b.table + p.s * b.table_stride;
+      pbase = p.key0 >> b.shift;
+      plast = (p.key1 - 1) >> b.shift;
+      ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
+      hoff = (p.block / a.HB) * b.head_stride;
+    };
+    auto issue = [&](int stage) {
+      if (p.x < p.x1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int tl = pt + u * G;  // first key of the step
+          if (tl < p.key1 && ((min(tl + G, p.key1) - 1) >> b.shift) >= pbase + 32) {  // warp-uniform
+            pbase = tl >> b.shift;
+            ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
+          }
+          const int t = tl + g;
+          const int id = __shfl_sync(kAll, ids, ((t >> b.shift) - pbase) & 31);
+          const bool in = t < p.key1, ok = (unsigned)id < (unsigned)b.n_pages;
+          const int64_t off =
+              in && ok ? id * b.page_stride + (int64_t)(t & ((1 << b.shift) - 1)) * b.slot_stride + hoff : 0;
+          const uint32_t dst = ring + (stage * U + u) * 1024;
+          copy16(dst, kb + off, in && ok);
+          copy16(dst + 512, vb + off, in && ok);
+          const uint32_t bit = 1u << (stage * U + u);
+          bad &= ~bit;
+          if (in && !ok) {
+            bad |= bit;
+            flag(b.status, kErrInput);
+          }
+        }
+        pt += S::KPI;
+        if (pt >= p.key1) {
+          p.next(b, KVB);
+          enter();
+        }
+      }
+      copy_commit();
+    };
+    enter();
+#pragma unroll
+    for (int i = 0; i < STG - 1; ++i) issue(i);
+    int stage = 0;
+    while (c.x < c.x1) {
+      const int key0 = c.key0, key1 = c.key1, s = c.s, block = c.block;
       const int kvh = block / a.HB, hb = block - kvh * a.HB;
       const int h0 = kvh * b.rep + hb * a.per;  // first query head of the block
       const int nr = min(a.per, b.rep - hb * a.per);
@@ -220,51 +323,17 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
-      const int32_t* row = b.table + s * b.table_stride;
-      const KT* kb = static_cast<const KT*>(b.k) + kvh * b.head_stride + li * EPL;
-      const KT* vb = static_cast<const KT*>(b.v) + kvh * b.head_stride + li * EPL;
-      // page ids: lane i holds the id of page pbase + i
-      int pbase = key0 >> b.shift;
-      const int plast = key1 > 0 ? (key1 - 1) >> b.shift : -1;
-      int ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
-      auto load = [&](int t0, uint4 (&kk)[U], uint4 (&vv)[U]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int tl = t0 + u * G;  // first key of the step
-          const int pg = (tl + g) >> b.shift;
-          if (tl < key1 && ((min(tl + G, key1) - 1) >> b.shift) >= pbase + 32) {  // warp-uniform
-            pbase = tl >> b.shift;
-            ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
-          }
-          const int id = __shfl_sync(kAll, ids, (pg - pbase) & 31);
-          kk[u] = vv[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (tl + g < key1) {
-            if ((unsigned)id < (unsigned)b.n_pages) {
-              const int64_t off = id * b.page_stride + (int64_t)((tl + g) & ((1 << b.shift) - 1)) * b.slot_stride;
-              kk[u] = __ldcs(reinterpret_cast<const uint4*>(kb + off));
-              vv[u] = __ldcs(reinterpret_cast<const uint4*>(vb + off));
-            } else {  // the row becomes NaN through its score
-              kk[u] = make_uint4(~0u, ~0u, ~0u, ~0u);
-              flag(b.status, kErrInput);
-            }
-          }
-        }
-      };
-      uint4 kn[U], vn[U];
-      if (key0 < key1) load(key0, kn, vn);
       for (int t0 = key0; t0 < key1; t0 += S::KPI) {
-        uint4 kc[U], vc[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          kc[u] = kn[u];
-          vc[u] = vn[u];
-        }
-        if (t0 + S::KPI < key1) load(t0 + S::KPI, kn, vn);
+        copy_wait<STG - 2>();
+        issue(stage == 0 ? STG - 1 : stage - 1);
+        const uint4* rg = ring_g + stage * U * 64;
         float sc[S::NV];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float2 kx[E2];
-          widen16(kc[u], kx);
+          uint4 kw = rg[u * 64];
+          if (bad >> (stage * U + u) & 1) kw = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN score, NaN row
+          widen16(kw, kx);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             float2 d = make_float2(0.f, 0.f);
@@ -274,16 +343,16 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
           }
         }
         // halving exchange over the key's lanes
-        int c = S::NV;
+        int cnt = S::NV;
 #pragma unroll
         for (int o = L / 2; o >= 1; o >>= 1) {
-          if (c > 1) {
-            c >>= 1;
+          if (cnt > 1) {
+            cnt >>= 1;
             const bool up = (lane & o) != 0;
 #pragma unroll
             for (int i = 0; i < S::NV / 2; ++i)
-              if (i < c) {
-                const float send = up ? sc[i] : sc[i + c], keep = up ? sc[i + c] : sc[i];
+              if (i < cnt) {
+                const float send = up ? sc[i] : sc[i + cnt], keep = up ? sc[i + cnt] : sc[i];
                 sc[i] = keep + __shfl_xor_sync(kAll, send, o);
               }
           } else {
@@ -333,7 +402,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float2 vx[E2];
-          widen16(vc[u], vx);
+          widen16(rg[u * 64 + 32], vx);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             constexpr int kDiv = NS;
@@ -344,6 +413,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
             for (int e = 0; e < E2; ++e) acc[r][e] = __ffma2_rn(p2, vx[e], acc[r][e]);
           }
         }
+        stage = stage + 1 == STG ? 0 : stage + 1;
       }
       // join the G groups: every lane ends with the item's m, l of its own heads
       float w[RL];
@@ -360,8 +430,15 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int o = L; o < 32; o <<= 1) l[i] += __shfl_xor_sync(kAll, l[i], o);
       }
-      const bool begin = u0 == 0, end = u1 == us;
-      float* slot = slots + (size_t)(2 * warp + (x == xb ? 0 : 1)) * S::STATE;
+      const bool begin = c.u0 == 0, end = c.u1 == c.us;
+      // (a last piece's slot lies in the ring: its loads have been consumed, but
+      // every lane has to be past its own)
+      const int which = c.x == xb ? 0 : 1;
+      float* slot = reinterpret_cast<float*>(mine + which * S::STATE * 4);
+      if (which) {
+        copy_wait<0>();
+        __syncwarp();
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int src = gbase + (r / RL) * DUP;
@@ -402,22 +479,15 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
           }
         }
       }
-      if (lane == 0 && !(begin && end)) segs[2 * warp + (x == xb ? 0 : 1)] = {first, s, block, 1, begin, end};
-      x += u1 - u0;
-      u0 = 0;
-      if (end && ++block == KVB) {
-        block = 0;
-        first += us;
-        ++s;
-        if (x < x1) {
-          keys = keys_of(b, s);
-          us = units_of<CH>(keys);
-        }
-      }
+      if (lane == 0 && !(begin && end)) segs[2 * warp + which] = {c.first, s, block, 1, begin, end};
+      c.next(b, KVB);
     }
   }
   __syncthreads();
   // ---- pieces of items inside this CTA, in order
+  auto state_of = [&](int k) {
+    return reinterpret_cast<const float*>(smem + (k >> 1) * S::WARP + (k & 1) * S::STATE * 4);
+  };
   if (threadIdx.x == 0) a.desc[blockIdx.x].z = 0;
   for (int i = 0; i < 2 * kDecodeWarps;) {
     if (!segs[i].valid) {
@@ -439,12 +509,12 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(DecodeArgs a) {
       const int r = x / HD;
       float M = -INFINITY;
       for (int k = i; k <= last; ++k)
-        if (segs[k].valid) M = fmaxf(M, slots[(size_t)k * S::STATE + R * HD + r]);
+        if (segs[k].valid) M = fmaxf(M, state_of(k)[R * HD + r]);
       const float ref = ref_of(M);
       float o = 0.f, lsum = 0.f;
       for (int k = i; k <= last; ++k)
         if (segs[k].valid) {
-          const float* p = slots + (size_t)k * S::STATE;
+          const float* p = state_of(k);
           const float w = ex2(p[R * HD + r] - ref);
           o += w * p[x];
           lsum += w * p[R * HD + R + r];
