@@ -3,7 +3,6 @@
 #include <math.h>
 
 #include "paged.cuh"
-#include "paged_decode.cuh"
 
 namespace q6w {
 namespace paged {
@@ -307,12 +306,10 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
     d.ldq = query_stride;
     d.out = output;
     d.H = n_heads;
-    d.HB = (a.b.rep + 7) / 8;
-    d.per = (a.b.rep + d.HB - 1) / d.HB;
+    d.hd = p->head_dim;
     d.scale = a.scale;
     d.desc = static_cast<int4*>(workspace);
-    d.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t)sm_count() * 64);
-    return decode_attention(d, p->head_dim, half, s);
+    return decode_attention(d, half, s);
   }
   switch (p->head_dim) {
     case 16: launch_rows<16>(a, half, s); break;

@@ -73,5 +73,24 @@ __device__ __forceinline__ int token_seq(const Batch& b, int t, int lane) {
   return lo - 1;
 }
 
+// ---- decode attention (paged_decode.cu) -------------------------------------
+
+struct DecodeArgs {
+  Batch b;
+  const float* q;
+  int64_t ldq;
+  float* out;
+  float* wpart;     // [warp of the grid][2][state]: pieces of items
+  float* part;      // [CTA][2][state]: pieces joined inside a CTA
+  int4* desc;       // [CTA]: item that starts in the CTA and goes on: {s, block, CTAs, 0}
+  int32_t H, HB, per;  // query heads, head blocks of a kv head, heads of a block
+  int32_t hd, F;       // head_dim, kv heads side by side
+  float scale;         // log2(e) / sqrt(head_dim)
+};
+
+// One query token a sequence; workspace (desc): decode_workspace bytes.
+int32_t decode_attention(const DecodeArgs& a, bool half, cudaStream_t st);
+size_t decode_workspace(int head_dim);
+
 }  // namespace paged
 }  // namespace q6w
