@@ -424,7 +424,8 @@ Q6W_API size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n
  * and a prompt's or a chunk's attention for more.  queries (rotated)
  * [n_tokens, n_heads, head_dim] FP32 with a token stride in elements
  * (a multiple of 4); output [n_tokens, n_heads, head_dim] contiguous.
- * n_heads is a multiple of kv_heads.  Scores, softmax and sums are FP32.  A
+ * n_heads is a multiple of kv_heads, and page_size * head_dim elements are
+ * at least 128 bytes.  Scores, softmax and sums are FP32.  A
  * token with no visible key (length 0, padding by length) gives zeros; rows
  * of tokens that no sequence holds are zeroed when zero_padding is set and
  * left as they were otherwise.  Slots behind a sequence's length may hold anything.  A row that

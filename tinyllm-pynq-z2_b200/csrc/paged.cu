@@ -228,6 +228,10 @@ static int32_t check_batch(const char* who, const q6w_paged_batch* p, int32_t n_
   if (p->page_stride % unit || p->slot_stride % unit || p->head_stride % unit || p->page_stride < 0 ||
       p->slot_stride < 0 || p->head_stride < 0)
     return fail(Q6W_ERR_ALIGN, "%s: page, slot and head strides must be multiples of 16 bytes", who);
+  // offsets inside a page are 32-bit in the kernels
+  const int64_t span = (p->page_size - 1) * p->slot_stride + (p->kv_heads - 1) * p->head_stride + hd;
+  if (p->slot_stride > (1 << 28) || p->head_stride > (1 << 28) || span > (1 << 28))
+    return fail(Q6W_ERR_ARG, "%s: a page spans more than 2^28 elements", who);
   if (n_tokens > 0 && p->n_seqs > 0) {
     if (!p->k_pages || !p->v_pages || !p->lengths || (p->max_pages > 0 && !p->page_table))
       return fail(Q6W_ERR_ARG, "%s: null pointer", who);
@@ -280,6 +284,8 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
   st = check_heads(who, p, n_heads, &a.b);
   if (st) return st;
   if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
+  if (p->page_size * p->head_dim * (p->kv_dtype == Q6W_KV_F16 ? 2 : 4) < 128)
+    return fail(Q6W_ERR_ARG, "%s: a kv head's part of a page must be at least 128 bytes", who);
   if (n_tokens == 0) return Q6W_OK;
   if (!queries || !output || (prefix_length > 0 && !prefix_pages)) return fail(Q6W_ERR_ARG, "%s: null pointer", who);
   if (!aligned(queries, 16) || !aligned(output, 16) || query_stride % 4)

@@ -85,6 +85,7 @@ struct DecodeArgs {
   int4* desc;       // [CTA]: item that starts in the CTA and goes on: {s, block, CTAs, 0}
   int32_t H, HB, per;  // query heads, head blocks of a kv head, heads of a block
   int32_t hd, F;       // head_dim, kv heads side by side
+  int32_t swap;        // the pool's map holds slots in front of kv heads
   float scale;         // log2(e) / sqrt(head_dim)
 };
 

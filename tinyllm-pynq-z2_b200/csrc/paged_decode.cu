@@ -36,6 +36,9 @@
 // balance alike.  A warp that holds an item whole writes its output; pieces
 // of an item go through the workspace, joined by their CTA when it holds them
 // all, else by merge_kernel.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -45,7 +48,7 @@
 namespace q6w {
 namespace paged {
 
-constexpr int kTile = 16;  // keys of a unit: one MMA's M side
+constexpr int kTile = 16;  // keys of an MMA's M side
 
 // A partial state: o[8][head_dim], m[8], l[8].
 __host__ __device__ constexpr int state_floats(int hd) { return 8 * hd + 16; }
@@ -57,25 +60,63 @@ __device__ __forceinline__ void block_heads(const DecodeArgs& a, int block, int&
   nr = a.F > 1 ? a.F * a.b.rep : min(a.per, a.b.rep - hb * a.per);
 }
 
-// Warps, shared-memory ring and CTAs an SM by the width HDF = F head_dim.
+// Shapes by the width HDF = F head_dim and the element size.
+//
+// Loads.  A tile (16 keys of one item: 16 rows of RB bytes) is one TMA box, or
+// 16 / page_size boxes of smaller pages, into a ring that the warp owns,
+// half units (keys, values, keys, ...) STG - 1 ahead of the arithmetic and
+// over the ends of items.  Lane-wise 16-byte copies of the same rows stopped at
+// 3.5 TB/s whatever the arithmetic (64- and 128-byte requests: the L1's
+// outstanding requests run out); one bulk copy a row at one row in 9 cycles
+// (4 TB/s at 128 bytes).
+// Rows arrive swizzled in 16-byte units by min(RB, 128) bytes; kappa(g) is the
+// key that stands in row g (g + 8: kappa(g) + 8) of the MMA's M side, chosen
+// for each RB so that neither the reads of K (rows g by quarter-warps) nor
+// those of V (rows of four lane columns) meet in a bank (RB 512: V two-way).
 template <int HDF, typename KT>
 struct DecodeShape {
   static constexpr int ES = (int)sizeof(KT);
-  static constexpr int CK = HDF / 4 * ES < 16 ? HDF / 4 * ES : 16;  // bytes of a lane's K chunk
-  static constexpr int CV = HDF / 8 * ES < 16 ? HDF / 8 * ES : 16;
-  static constexpr int NK = HDF / 4 * ES / CK;  // K chunks of a key that a lane holds (4 lanes a key)
-  static constexpr int NVC = HDF / 8 * ES / CV; // V chunks of a key that a lane holds (8 lanes a key)
+  static constexpr int RB = HDF * ES;                               // bytes of a key's row
+  static constexpr int IB = RB < 128 ? RB : 128;                    // inner box bytes = swizzle span
+  static constexpr int CK = RB / 4 < 16 ? RB / 4 : 16;  // bytes of a lane's K chunk
+  static constexpr int CV = RB / 8 < 16 ? RB / 8 : 16;
+  static constexpr int NK = RB / 4 / CK;   // K chunks of a key that a lane holds (4 lanes a key)
+  static constexpr int NVC = RB / 8 / CV;  // V chunks of a key that a lane holds (8 lanes a key)
   static constexpr int EK = CK / ES, EV = CV / ES;
-  static constexpr int HALF = kTile * HDF * ES;  // bytes of a unit's keys (or values)
-  // The loads run ahead in a ring of half units (K and V alternate).  HDF 128
-  // FP32 needs 64 + 32 registers for q and o: one CTA an SM; else two.
-  static constexpr int CTAS = HDF >= 128 ? 1 : 2;
-  static constexpr int kMost = (CTAS == 1 ? 24 : 12) * 1024 / HALF;
+  // Tiles of a unit: two where the registers allow it, so that the checks, the
+  // joining of a tile's output and the loop itself are paid half as often.
+  static constexpr int NT = RB <= 128 ? 2 : 1;
+  static constexpr int KU = NT * kTile;  // keys of a unit
+  static constexpr int TILE = kTile * RB;
+  static constexpr int HALF = NT * TILE;  // bytes of a unit's keys (or values)
+  // CTAs of four warps an SM, by registers (255, 168, 128 a thread); 192 KB of rings an SM
+  static constexpr int CTAS = HDF >= 128 ? 2 : HDF >= 64 ? 3 : 4;
+  static constexpr int kMost = 48 / CTAS * 1024 / HALF;
   static constexpr int STG = kMost < 8 ? kMost : 8;
   static constexpr int RING = STG * HALF;
+  __device__ static __forceinline__ int kappa(int g) {
+    if (ES == 2) {
+      if (RB == 128) return g ^ ((g & 1) << 2);
+      if (RB == 64) return ((g & 4) | ((g >> 1) & 1)) ^ ((g & 1) * 3);
+      return (g >> 1) ^ ((g & 1) * 6);
+    }
+    if (RB == 64) return (g & 1) | ((g & 2) << 1) | ((g & 4) >> 1);
+    if (RB == 128) return ((g & 1) << 2) | (g & 2) | ((g & 4) >> 2);
+    if (RB == 256) return (g & 4) | ((g & 1) << 1) | ((g >> 1) & 1);
+    return g;
+  }
+  // Byte place of byte `at` of row `row` of a tile.
+  __device__ static __forceinline__ int place(int row, int at) {
+    const int x = row * RB + at;
+    return IB == 128 ? x ^ ((x >> 3) & 0x70) : IB == 64 ? x ^ ((x >> 3) & 0x30) : x ^ ((x >> 3) & 0x10);
+  }
 };
 
-constexpr int kDecodeWarps = 8;
+struct DecodeMaps {
+  CUtensorMap k, v;
+};
+
+constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -101,8 +142,12 @@ struct Line {
 // Keys that sequence s's token sees.
 __device__ __forceinline__ int keys_of(const Batch& b, int s) { return min(max(__ldg(b.lengths + s), 0), b.max_len); }
 
-__device__ __forceinline__ int units_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
+template <int KU>
+__device__ __forceinline__ int units_of(int keys) {
+  return max(1, (keys + KU - 1) / KU);
+}
 
+template <int KU>
 __device__ __forceinline__ void build_line(const Batch& b, Line& line) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (b.n + kDecodeThreads - 1) / kDecodeThreads;
@@ -110,7 +155,7 @@ __device__ __forceinline__ void build_line(const Batch& b, Line& line) {
   for (int s = tid * seg; s < min((tid + 1) * seg, b.n); ++s) {
     const int len = __ldg(b.lengths + s);
     if (len > b.max_len) flag(b.status, kErrInput);
-    sum += units_of(min(max(len, 0), b.max_len));
+    sum += units_of<KU>(min(max(len, 0), b.max_len));
   }
   int64_t incl = sum;
 #pragma unroll
@@ -132,6 +177,7 @@ __device__ __forceinline__ void build_line(const Batch& b, Line& line) {
 }
 
 // Sequence that holds unit z (counted without head blocks), and its first unit.
+template <int KU>
 __device__ __forceinline__ void find_seq(const Batch& b, const Line& line, int64_t z, int lane, int& s, int64_t& first) {
   int c = 0;
 #pragma unroll
@@ -143,7 +189,7 @@ __device__ __forceinline__ void find_seq(const Batch& b, const Line& line, int64
   first = line.pref[c - 1];
   for (;;) {
     const int i = s + lane;
-    const int u = i < b.n ? units_of(keys_of(b, i)) : 0;
+    const int u = i < b.n ? units_of<KU>(keys_of(b, i)) : 0;
     int64_t incl = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -166,13 +212,14 @@ struct Seg {
 };
 
 // A warp's place on the line: the piece [u0, u1) of an item.
+template <int KU>
 struct Cursor {
   int64_t x, x1, first;
   int s, block, keys, us, u0, u1, key0, key1;
   __device__ __forceinline__ void piece() {
     u1 = (int)min((int64_t)us, u0 + (x1 - x));
-    key0 = u0 * kTile;
-    key1 = min(u1 * kTile, keys);
+    key0 = u0 * KU;
+    key1 = min(u1 * KU, keys);
   }
   __device__ __forceinline__ void next(const Batch& b, int KVB) {
     x += u1 - u0;
@@ -183,26 +230,20 @@ struct Cursor {
       ++s;
       if (x < x1) {
         keys = keys_of(b, s);
-        us = units_of(keys);
+        us = units_of<KU>(keys);
       }
     }
     piece();
   }
 };
 
-// Bytes from global to shared memory, zeros instead when `in` is false.
-template <int N>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool in) {
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(in ? N : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A box of the pool: coordinates (element, segment, then kv-head block and slot in the map's order, page).
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int c2, int c3, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c2), "r"(c3), "r"(page), "r"(smem_u32(bar))
+      : "memory");
 }
 
 // N bytes of shared memory as 32-bit words.
@@ -219,22 +260,31 @@ __device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&w)[N / 4
   }
 }
 
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c; `first` (a constant): c is zero.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+// Transpose of an 8 x 8 matrix of 16-bit values held as MMA fragments.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
-// x = hi + lo, two TF32 values: hi rounded to nearest (11 bits), lo the rest cut
-// to 11 bits.  A NaN stays one in lo.
+// x = hi + lo as TF32 operands: hi rounded to nearest (11 bits), lo the exact
+// rest, of which the MMA takes the upper 11 bits.  A NaN stays one in lo.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = (x + 0x1000u) & 0xffffe000u;
-  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
 // (x, y) -> their FP16 parts hi and lo, packed.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -246,22 +296,28 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
 }
 
 template <int HDF, typename KT>
-__global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) decode_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
+    decode_kernel(DecodeArgs a, const __grid_constant__ DecodeMaps maps) {
   using S = DecodeShape<HDF, KT>;
   constexpr bool kHalf = std::is_same<KT, __half>::value;
   constexpr int NK = S::NK, NVC = S::NVC, EK = S::EK, EV = S::EV, CK = S::CK, CV = S::CV, STG = S::STG;
+  constexpr int NT = S::NT;                  // tiles of a unit
   constexpr int MT = HDF / 16;               // M tiles of O^T
   constexpr int QS = kHalf ? HDF / 16 : HDF / 8;  // K steps of S
   constexpr float kOff = kHalf ? 4.f : 0.f;  // FP16 weights reach 2^(kOff + 8): their low parts stay normal
   constexpr unsigned kAll = 0xffffffffu;
-  extern __shared__ __align__(16) uint8_t smem[];  // [warp][RING]
+  extern __shared__ uint8_t smem_raw[];  // [warp][RING], 1024-byte aligned
+  __shared__ uint64_t bars[kDecodeWarps * STG];
   __shared__ Line line;
   __shared__ Seg segs[2 * kDecodeWarps];
   const Batch& b = a.b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;  // the MMA fragments' row group and column group
   const int STATE = state_floats(a.hd);
-  build_line(b, line);
+  uint64_t* bar = bars + warp * STG;
+  if (lane < STG) mbar_init(bar + lane, 1);
+  fence_mbar_init();
+  build_line<S::KU>(b, line);
   const int KVB = b.kv_heads / a.F * a.HB;
   const int64_t units = line.total * KVB;
   // few units: spread them over the CTAs first, over a CTA's warps second
@@ -272,34 +328,27 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
   if (lane < 2) segs[2 * warp + lane].valid = 0;
   float* slots = a.wpart + ((size_t)blockIdx.x * kDecodeWarps + warp) * 2 * STATE;
   if (active) {
-    Cursor cur;
+    Cursor<S::KU> cur;
     cur.x = wi * units / workers;
     cur.x1 = (wi + 1) * units / workers;
     const int64_t xb = cur.x;
-    find_seq(b, line, cur.x / KVB, lane, cur.s, cur.first);
+    find_seq<S::KU>(b, line, cur.x / KVB, lane, cur.s, cur.first);
     cur.keys = keys_of(b, cur.s);
-    cur.us = units_of(cur.keys);
+    cur.us = units_of<S::KU>(cur.keys);
     cur.block = (int)((cur.x - cur.first * KVB) / cur.us);
     cur.u0 = (int)((cur.x - cur.first * KVB) % cur.us);
     cur.piece();
 
-    // ---- loads: half units in consumption order (keys, values, keys, ...),
-    // over the ends of items, into a ring that is private to each lane (a lane
-    // reads the bytes that it copied itself: waiting for its own copies is
-    // enough).  Lane (g, c) takes of keys g and g + 8 dims j 4 EK + c EK + e
-    // (j < NK, e < EK), of the values of its four keys dims j 8 EV + g EV + e.
-    const uint8_t* ring_g = smem + warp * S::RING;
-    const uint32_t ring = smem_u32(ring_g);
-    Cursor p = cur;
-    const KT* kbase = static_cast<const KT*>(b.k);
-    const KT* vbase = static_cast<const KT*>(b.v);
-    const bool one_page = b.shift >= 4;  // a unit lies inside a page
+    // ---- loads
+    const uint32_t ring = ((smem_u32(smem_raw) + 1023) & ~1023u) + warp * S::RING;
+    const uint8_t* ring_g = smem_raw + (ring - smem_u32(smem_raw));
+    Cursor<S::KU> p = cur;
+    const int boxes = b.shift >= 4 ? 1 : kTile >> b.shift;  // boxes of a tile
+    const int slot_mask = (1 << b.shift) - 1;
     const int32_t* row = b.table;
     int pt = 0, pbase = 0, plast = -1, ids = -1;  // page ids: lane i holds the id of page pbase + i
-    int64_t hoff = 0;
     int istage = 0;
-    uint32_t bad = 0;  // bits 2 stage, 2 stage + 1: key g, key g + 8 has a page id out of range
-    auto value_key = [&](int i) { return kHalf ? 2 * c + (i & 1) + 8 * (i >> 1) : c + 4 * i; };
+    uint32_t bad = 0;  // bits 2 stage + tile: the tile has a page id out of range
     auto enter = [&]() {  // the first piece from p on that has keys
       while (p.x < p.x1 && p.key0 >= p.key1) p.next(b, KVB);
       if (p.x >= p.x1) return;
@@ -308,51 +357,38 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
       pbase = p.key0 >> b.shift;
       plast = (p.key1 - 1) >> b.shift;
       ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
-      hoff = (int64_t)(p.block / a.HB) * a.F * b.head_stride;
     };
-    // offset of key t (any lane's), by the whole warp; -1: a bad page id
-    auto offset = [&](int t) -> int64_t {
-      const int id = __shfl_sync(kAll, ids, ((t >> b.shift) - pbase) & 31);
-      if ((unsigned)id >= (unsigned)b.n_pages) return -1;
-      return id * b.page_stride + (int64_t)(t & ((1 << b.shift) - 1)) * b.slot_stride + hoff;
-    };
+    // Start the next half unit's copies.  Lane t boxes + i starts box i of tile t.
     auto issue = [&](bool values) {
       if (p.x < p.x1) {
-        const uint32_t dst = ring + istage * S::HALF;
-        if (((min(pt + kTile, p.key1) - 1) >> b.shift) >= pbase + 32) {  // warp-uniform
+        const int t = lane / boxes, i = lane - t * boxes;
+        const int first = pt + t * kTile + (i << b.shift);  // the box's first key
+        // (a unit's pages are the lanes' or the next 32: both are aligned to the unit)
+        if (!values && ((min(pt + S::KU, p.key1) - 1) >> b.shift) >= pbase + 32) {
           pbase = pt >> b.shift;
           ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
         }
-        const int64_t base = one_page ? offset(pt) : 0;
+        const int id = __shfl_sync(kAll, ids, ((first >> b.shift) - pbase) & 31);
+        const bool in = t < NT && first < p.key1, ok = (unsigned)id < (unsigned)b.n_pages;
+        const int count = __popc(__ballot_sync(kAll, in && ok));
         if (!values) {
+          const unsigned wrong = __ballot_sync(kAll, in && !ok);
           bad &= ~(3u << (2 * istage));
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int k = g + 8 * r;
-            int64_t off = one_page ? (base < 0 ? base : base + k * b.slot_stride) : offset(pt + k);
-            const bool in = pt + k < p.key1;
-            if (in && off < 0) {
-              bad |= 1u << (2 * istage + r);
-              flag(b.status, kErrInput);
-            }
-            const bool ok = in && off >= 0;
-            if (!ok) off = 0;
-#pragma unroll
-            for (int j = 0; j < NK; ++j)
-              copy_async<CK>(dst + ((r * NK + j) * 32 + lane) * CK, kbase + off + j * 4 * EK + c * EK, ok);
+          if (wrong) {
+            const uint32_t one = (1u << boxes) - 1u;
+            bad |= ((wrong & one ? 1u : 0u) | (NT == 2 && (wrong >> boxes) & one ? 2u : 0u)) << (2 * istage);
+            if (lane == 0) flag(b.status, kErrInput);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = value_key(i);
-            int64_t off = one_page ? (base < 0 ? base : base + k * b.slot_stride) : offset(pt + k);
-            const bool ok = pt + k < p.key1 && off >= 0;
-            if (!ok) off = 0;
-#pragma unroll
-            for (int j = 0; j < NVC; ++j)
-              copy_async<CV>(dst + ((i * NVC + j) * 32 + lane) * CV, vbase + off + j * 8 * EV + g * EV, ok);
-          }
-          pt += kTile;
+        }
+        if (lane == 0) mbar_expect_tx(bar + istage, count * (S::TILE / boxes));
+        __syncwarp();
+        if (in && ok) {
+          const int blk = p.block / a.HB, slot = first & slot_mask;
+          load_box(ring + istage * S::HALF + t * S::TILE + i * (S::TILE / boxes), values ? &maps.v : &maps.k,
+                   a.swap ? slot : blk, a.swap ? blk : slot, id, bar + istage);
+        }
+        if (values) {
+          pt += S::KU;
           if (pt >= p.key1) {
             p.next(b, KVB);
             enter();
@@ -360,24 +396,32 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
         }
       }
       istage = istage + 1 == STG ? 0 : istage + 1;
-      copy_commit();
     };
     enter();
-    bool next_values = false;
-#pragma unroll
-    for (int i = 0; i < STG - 1; ++i) {
-      issue(next_values);
-      next_values = !next_values;
-    }
+#pragma unroll 1
+    for (int i = 0; i < STG - 1; ++i) issue(i & 1);
     int stage = 0;
-    auto advance = [&]() {  // the oldest half unit is here; start the load that takes the place of the one before it
-      copy_wait<STG - 2>();
-      issue(next_values);
-      next_values = !next_values;
+    uint32_t phase = 0;
+    bool late = false;  // a wait ran out: the warp's outputs become NaN
+    // Wait for the oldest half unit, and start the load that takes the place of
+    // the one before it (which every lane has read), STG - 1 halves ahead.
+    auto advance = [&](bool values) {
+      if (!mbar_wait(bar + stage, phase)) late = true;
+      __syncwarp();
+      issue(values != ((STG - 1) % 2 != 0));
       const uint8_t* at = ring_g + stage * S::HALF;
-      stage = stage + 1 == STG ? 0 : stage + 1;
+      if (++stage == STG) {
+        stage = 0;
+        phase ^= 1;
+      }
       return at;
     };
+    // the lane's places in a tile: K chunk j of row kappa(g) + 8 r, V chunk j of
+    // its value key i (the rows that P^T's fragments hold)
+    const int krow = S::kappa(g);
+    int vrow[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vrow[i] = S::kappa(kHalf ? 2 * c + (i & 1) : c + 4 * (i & 1)) + 8 * (i >> 1);
 
     while (cur.x < cur.x1) {
       const int key0 = cur.key0, key1 = cur.key1, s = cur.s;
@@ -426,66 +470,77 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
       float acc[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-      // heads 2 c and 2 c + 1: reference (0 until a score was seen), the score that moves it, sum
-      float ref0 = 0.f, ref1 = 0.f, top0 = -INFINITY, top1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-      for (int t0 = key0; t0 < key1; t0 += kTile) {
-        // ---- S^T = K q^T
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+      // heads 2 c and 2 c + 1: reference (0 until a score was seen), how far a
+      // score may pass it, sum of weights
+      float ref0 = 0.f, ref1 = 0.f, lim0 = -INFINITY, lim1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int t0 = key0; t0 < key1; t0 += S::KU) {
+        // ---- S^T = K q^T: key g heads 2 c, 2 c + 1, then key g + 8
+        float x[NT][4];
         {
-          const uint32_t nan2 = bad >> (2 * stage);
-          const uint8_t* kr = advance() + lane * CK;
+          const uint32_t nans = bad >> (2 * stage);
+          const uint8_t* kr = advance(false);
 #pragma unroll
-          for (int j = 0; j < NK; ++j) {
-            uint32_t w0[CK / 4], w1[CK / 4];  // keys g and g + 8
-            read_words<CK>(kr + j * 32 * CK, w0);
-            read_words<CK>(kr + (NK + j) * 32 * CK, w1);
-            if (j == 0) {
-              if (nan2 & 1) w0[0] = ~0u;
-              if (nan2 & 2) w1[0] = ~0u;
-            }
+          for (int t = 0; t < NT; ++t) {
+            float s0[4], s1[4], s2[4];
 #pragma unroll
-            for (int h = 0; h < CK / 8; ++h) {
-              const int st = j * (CK / 8) + h;
-              if constexpr (kHalf) {
-                const uint32_t ka[4] = {w0[2 * h], w1[2 * h], w0[2 * h + 1], w1[2 * h + 1]};
-                mma_f16(s0, ka, qhi[2 * st], qhi[2 * st + 1]);
-                mma_f16(s1, ka, qlo[2 * st], qlo[2 * st + 1]);
-              } else {
-                uint32_t kh[4], kl[4];
-                split_tf32(w0[2 * h], kh[0], kl[0]);
-                split_tf32(w1[2 * h], kh[1], kl[1]);
-                split_tf32(w0[2 * h + 1], kh[2], kl[2]);
-                split_tf32(w1[2 * h + 1], kh[3], kl[3]);
-                mma_tf32(s0, kh, qhi[2 * st], qhi[2 * st + 1]);
-                mma_tf32(s1, kh, qlo[2 * st], qlo[2 * st + 1]);
-                mma_tf32(s2, kl, qhi[2 * st], qhi[2 * st + 1]);
+            for (int j = 0; j < NK; ++j) {
+              uint32_t w0[CK / 4], w1[CK / 4];  // keys g and g + 8
+              read_words<CK>(kr + t * S::TILE + S::place(krow, j * 4 * CK + c * CK), w0);
+              read_words<CK>(kr + t * S::TILE + S::place(krow + 8, j * 4 * CK + c * CK), w1);
+#pragma unroll
+              for (int h = 0; h < CK / 8; ++h) {
+                const int st = j * (CK / 8) + h;
+                if constexpr (kHalf) {
+                  const uint32_t ka[4] = {w0[2 * h], w1[2 * h], w0[2 * h + 1], w1[2 * h + 1]};
+                  mma_f16(s0, ka, qhi[2 * st], qhi[2 * st + 1], st == 0);
+                  mma_f16(s1, ka, qlo[2 * st], qlo[2 * st + 1], st == 0);
+                } else {
+                  uint32_t kh[4], kl[4];
+                  split_tf32(w0[2 * h], kh[0], kl[0]);
+                  split_tf32(w1[2 * h], kh[1], kl[1]);
+                  split_tf32(w0[2 * h + 1], kh[2], kl[2]);
+                  split_tf32(w1[2 * h + 1], kh[3], kl[3]);
+                  mma_tf32(s0, kh, qhi[2 * st], qhi[2 * st + 1], st == 0);
+                  mma_tf32(s1, kh, qlo[2 * st], qlo[2 * st + 1], st == 0);
+                  mma_tf32(s2, kl, qhi[2 * st], qhi[2 * st + 1], st == 0);
+                }
               }
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][i] = kHalf ? s0[i] + s1[i] : s0[i] + (s1[i] + s2[i]);
+            if (nans >> t & 1) x[t][0] = x[t][1] = x[t][2] = x[t][3] = NAN;  // never loaded: NaN rows
           }
         }
-        // ---- weights: x0, x1 of key g (heads 2 c, 2 c + 1), x2, x3 of key g + 8
-        float x0 = (s0[0] + (s1[0] + s2[0])) * sc0, x1 = (s0[1] + (s1[1] + s2[1])) * sc1;
-        float x2 = (s0[2] + (s1[2] + s2[2])) * sc0, x3 = (s0[3] + (s1[3] + s2[3])) * sc1;
-        if (t0 + kTile > key1) {
-          if (t0 + g >= key1) x0 = x1 = -INFINITY;
-          if (t0 + g + 8 >= key1) x2 = x3 = -INFINITY;
+        if (t0 + S::KU > key1) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (t0 + t * kTile + krow >= key1) x[t][0] = x[t][1] = -INFINITY;
+            if (t0 + t * kTile + krow + 8 >= key1) x[t][2] = x[t][3] = -INFINITY;
+          }
         }
-        if (__any_sync(kAll, fmaxf(x0, x2) > top0 || fmaxf(x1, x3) > top1)) {
-          float m0 = fmaxf(x0, x2), m1 = fmaxf(x1, x3);
+        // ---- the references, when a score passes them by too much
+        float m0 = fmaxf(x[0][0], x[0][2]), m1 = fmaxf(x[0][1], x[0][3]);
+        if constexpr (NT == 2) {
+          m0 = fmaxf(m0, fmaxf(x[1][0], x[1][2]));
+          m1 = fmaxf(m1, fmaxf(x[1][1], x[1][3]));
+        }
+        m0 *= sc0;
+        m1 *= sc1;
+        if (__any_sync(kAll, m0 - ref0 > lim0 || m1 - ref1 > lim1)) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(kAll, m0, o));
             m1 = fmaxf(m1, __shfl_xor_sync(kAll, m1, o));
           }
-          // a head that has seen nothing yet has l = o = 0: any factor will do
-          m0 = fmaxf(m0, top0 == -INFINITY ? -INFINITY : ref0 + kOff);
-          m1 = fmaxf(m1, top1 == -INFINITY ? -INFINITY : ref1 + kOff);
-          const float n0 = m0 == -INFINITY ? 0.f : m0 - kOff, n1 = m1 == -INFINITY ? 0.f : m1 - kOff;
-          const float f0 = top0 == -INFINITY ? 1.f : ex2(ref0 - n0), f1 = top1 == -INFINITY ? 1.f : ex2(ref1 - n1);
+          // (a head that has seen nothing has l = o = 0: any factor will do)
+          const bool seen0 = lim0 != -INFINITY, seen1 = lim1 != -INFINITY;
+          const float n0 = seen0 ? fmaxf(m0 - kOff, ref0) : (m0 == -INFINITY ? 0.f : m0 - kOff);
+          const float n1 = seen1 ? fmaxf(m1 - kOff, ref1) : (m1 == -INFINITY ? 0.f : m1 - kOff);
+          const float f0 = seen0 ? ex2(ref0 - n0) : 1.f, f1 = seen1 ? ex2(ref1 - n1) : 1.f;
+          if (m0 != -INFINITY) lim0 = kOff + 8.f;
+          if (m1 != -INFINITY) lim1 = kOff + 8.f;
           ref0 = n0;
           ref1 = n1;
-          top0 = m0 + 8.f;
-          top1 = m1 + 8.f;
           l0 *= f0;
           l1 *= f1;
 #pragma unroll
@@ -496,87 +551,81 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
             acc[i][3] *= f1;
           }
         }
-        x0 = ex2(x0 - ref0);
-        x1 = ex2(x1 - ref1);
-        x2 = ex2(x2 - ref0);
-        x3 = ex2(x3 - ref1);
-        l0 += x0 + x2;
-        l1 += x1 + x3;
-        // ---- P^T as the MMA's B side: head g, the lane's four keys
-        float pv[4];
-        {
-          const bool odd = g & 1;
+        // ---- weights, and P^T as the MMA's B side: head g, the lane's four value keys
+        uint32_t phi[NT][4], plo[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float x0 = ex2(fmaf(x[t][0], sc0, -ref0)), x1 = ex2(fmaf(x[t][1], sc1, -ref1));
+          const float x2 = ex2(fmaf(x[t][2], sc0, -ref0)), x3 = ex2(fmaf(x[t][3], sc1, -ref1));
+          l0 += x0 + x2;
+          l1 += x1 + x3;
           if constexpr (kHalf) {
-            const int sa = 8 * c + (g >> 1), sb = sa + 4;  // lanes that hold keys 2 c (2 c + 8), 2 c + 1 (2 c + 9)
-            const float a0 = __shfl_sync(kAll, x0, sa), a1 = __shfl_sync(kAll, x1, sa);
-            const float b0 = __shfl_sync(kAll, x0, sb), b1 = __shfl_sync(kAll, x1, sb);
-            const float c0 = __shfl_sync(kAll, x2, sa), c1 = __shfl_sync(kAll, x3, sa);
-            const float d0 = __shfl_sync(kAll, x2, sb), d1 = __shfl_sync(kAll, x3, sb);
-            pv[0] = odd ? a1 : a0;
-            pv[1] = odd ? b1 : b0;
-            pv[2] = odd ? c1 : c0;
-            pv[3] = odd ? d1 : d0;
+            split_f16(x0, x1, phi[t][0], plo[t][0]);
+            split_f16(x2, x3, phi[t][1], plo[t][1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              phi[t][i] = transpose8(phi[t][i]);
+              plo[t][i] = transpose8(plo[t][i]);
+            }
           } else {
-            const int sa = 4 * c + (g >> 1), sb = sa + 16;  // keys c (c + 8), c + 4 (c + 12)
+            const bool odd = g & 1;
+            const int sa = 4 * c + (g >> 1), sb = sa + 16;  // lanes that hold rows c (c + 8), c + 4 (c + 12)
             const float a0 = __shfl_sync(kAll, x0, sa), a1 = __shfl_sync(kAll, x1, sa);
             const float b0 = __shfl_sync(kAll, x0, sb), b1 = __shfl_sync(kAll, x1, sb);
             const float c0 = __shfl_sync(kAll, x2, sa), c1 = __shfl_sync(kAll, x3, sa);
             const float d0 = __shfl_sync(kAll, x2, sb), d1 = __shfl_sync(kAll, x3, sb);
-            pv[0] = odd ? a1 : a0;
-            pv[1] = odd ? b1 : b0;
-            pv[2] = odd ? c1 : c0;
-            pv[3] = odd ? d1 : d0;
+            split_tf32(__float_as_uint(odd ? a1 : a0), phi[t][0], plo[t][0]);
+            split_tf32(__float_as_uint(odd ? b1 : b0), phi[t][1], plo[t][1]);
+            split_tf32(__float_as_uint(odd ? c1 : c0), phi[t][2], plo[t][2]);
+            split_tf32(__float_as_uint(odd ? d1 : d0), phi[t][3], plo[t][3]);
           }
         }
         // ---- O^T += V^T P^T; M row g of tile i is the lane's dim 2 i, row g + 8 its dim 2 i + 1
         {
-          const uint8_t* vr = advance() + lane * CV;
-          uint32_t phi[4], plo[4];
-          if constexpr (kHalf) {
-            split_f16(pv[0], pv[1], phi[0], plo[0]);
-            split_f16(pv[2], pv[3], phi[1], plo[1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) split_tf32(__float_as_uint(pv[i]), phi[i], plo[i]);
-          }
+          const uint8_t* vr = advance(true);
+          const bool tail = t0 + S::KU > key1;  // slots behind the last key may hold anything
 #pragma unroll
           for (int j = 0; j < NVC; ++j) {
-            uint32_t w[4][CV / 4];
+            float o[CV / S::ES / 2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) read_words<CV>(vr + (i * NVC + j) * 32 * CV, w[i]);
-            if constexpr (kHalf) {
+            for (int t = 0; t < NT; ++t) {
+              uint32_t w[4][CV / 4];
 #pragma unroll
-              for (int k = 0; k < CV / 4; ++k) {
-                const uint32_t va[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
-                                        __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
-                float o[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(o, va, plo[0], plo[1]);
-                mma_f16(o, va, phi[0], phi[1]);
-                const int i = j * (CV / 4) + k;
+              for (int i = 0; i < 4; ++i) read_words<CV>(vr + t * S::TILE + S::place(vrow[i], j * 8 * CV + g * CV), w[i]);
+              if (tail) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[i][x] += o[x];
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int k = 0; k < CV / 4; ++k)
+                    if (t0 + t * kTile + vrow[i] >= key1) w[i][k] = 0u;
               }
-            } else {
 #pragma unroll
-              for (int k = 0; k < CV / 8; ++k) {
-                float o[4] = {0.f, 0.f, 0.f, 0.f};
+              for (int k = 0; k < EV / 2; ++k) {
+                if constexpr (kHalf) {
+                  const uint32_t va[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                                          __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+                  mma_f16(o[k], va, plo[t][0], plo[t][1], t == 0);
+                  mma_f16(o[k], va, phi[t][0], phi[t][1], false);
+                } else {
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                  // K slots c, c + 4 of step kk: keys c + 8 kk, c + 8 kk + 4
-                  uint32_t vh[4], vl[4];
-                  split_tf32(w[2 * kk][2 * k], vh[0], vl[0]);
-                  split_tf32(w[2 * kk][2 * k + 1], vh[1], vl[1]);
-                  split_tf32(w[2 * kk + 1][2 * k], vh[2], vl[2]);
-                  split_tf32(w[2 * kk + 1][2 * k + 1], vh[3], vl[3]);
-                  mma_tf32(o, vl, phi[2 * kk], phi[2 * kk + 1]);
-                  mma_tf32(o, vh, plo[2 * kk], plo[2 * kk + 1]);
-                  mma_tf32(o, vh, phi[2 * kk], phi[2 * kk + 1]);
+                  for (int kk = 0; kk < 2; ++kk) {
+                    // K slots c, c + 4 of step kk: rows c + 8 kk, c + 8 kk + 4
+                    uint32_t vh[4], vl[4];
+                    split_tf32(w[2 * kk][2 * k], vh[0], vl[0]);
+                    split_tf32(w[2 * kk][2 * k + 1], vh[1], vl[1]);
+                    split_tf32(w[2 * kk + 1][2 * k], vh[2], vl[2]);
+                    split_tf32(w[2 * kk + 1][2 * k + 1], vh[3], vl[3]);
+                    mma_tf32(o[k], vl, phi[t][2 * kk], phi[t][2 * kk + 1], t == 0 && kk == 0);
+                    mma_tf32(o[k], vh, plo[t][2 * kk], plo[t][2 * kk + 1], false);
+                    mma_tf32(o[k], vh, phi[t][2 * kk], phi[t][2 * kk + 1], false);
+                  }
                 }
-                const int i = j * (CV / 8) + k;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) acc[i][x] += o[x];
               }
             }
+#pragma unroll
+            for (int k = 0; k < EV / 2; ++k)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[j * (EV / 2) + k][i] += o[k][i];
           }
         }
       }
@@ -586,6 +635,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
         l0 += __shfl_xor_sync(kAll, l0, o);
         l1 += __shfl_xor_sync(kAll, l1, o);
       }
+      if (late) l0 = l1 = NAN;
       const bool begin = cur.u0 == 0, end = cur.u1 == cur.us, whole = begin && end;
       const int which = cur.x == xb ? 0 : 1;
       float* slot = slots + which * STATE;
@@ -609,12 +659,16 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
           }
         }
         if (!whole && g == 0) {
-          slot[8 * a.hd + n] = (hh ? top1 : top0) == -INFINITY ? -INFINITY : (hh ? ref1 : ref0);
+          slot[8 * a.hd + n] = (hh ? lim1 : lim0) == -INFINITY ? -INFINITY : (hh ? ref1 : ref0);
           slot[8 * a.hd + 8 + n] = l;
         }
       }
       if (lane == 0 && !whole) segs[2 * warp + which] = {cur.first, s, cur.block, 1, begin, end};
       cur.next(b, KVB);
+    }
+    if (late) {  // the copies that are still on their way land before the CTA ends
+      if (lane == 0) flag(b.status, kErrTimeout);
+      for (int i = 0; i < STG; ++i) mbar_wait(bar + i, phase);
     }
   }
   __syncthreads();
@@ -664,7 +718,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS) de
     }
     if (threadIdx.x == 0 && f.begin && !end) {
       // the CTA that holds the item's last unit
-      const int us = units_of(keys_of(b, f.s));
+      const int us = units_of<S::KU>(keys_of(b, f.s));
       const int64_t lastu = f.first * KVB + (int64_t)(f.block + 1) * us - 1;
       const int c1 = (int)(owner_of(lastu, units, workers) / aw);
       a.desc[blockIdx.x] = make_int4(f.s, f.block, c1 - (int)blockIdx.x + 1, 0);
@@ -721,7 +775,7 @@ __global__ void __launch_bounds__(128) merge_kernel(DecodeArgs a) {
 
 // ---- host ---------------------------------------------------------------------
 
-constexpr int kMaxPerSm = 2;  // CTAs an SM at most (DecodeShape::CTAS)
+constexpr int kMaxPerSm = 4;  // CTAs an SM at most (DecodeShape::CTAS)
 
 // desc | CTA pieces | warp pieces
 size_t decode_workspace(int hd) {
@@ -729,11 +783,55 @@ size_t decode_workspace(int hd) {
   return ctas * (sizeof(int4) + (2 + 2 * kDecodeWarps) * state_floats(hd) * sizeof(float));
 }
 
+static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// The pool as (ib bytes, segments, kv-head blocks, slots, pages) -- blocks and
+// slots in ascending order of their strides -- with a box of `rows` slots of
+// one block.
+int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, CUtensorMap* map, bool* swap) {
+  auto encode = map_encoder();
+  if (!encode) return fail(Q6W_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const int rb = F * hd * es, ib = rb < 128 ? rb : 128;
+  const int page = 1 << b.shift;
+  cuuint64_t dim[5] = {(cuuint64_t)(ib / es), (cuuint64_t)(rb / ib), (cuuint64_t)(b.kv_heads / F), (cuuint64_t)page,
+                       (cuuint64_t)std::max(b.n_pages, 1)};
+  // (a dimension of one has no stride of its own)
+  const cuuint64_t ss = page > 1 ? (cuuint64_t)b.slot_stride * es : rb;
+  const cuuint64_t hs = b.kv_heads / F > 1 ? (cuuint64_t)F * b.head_stride * es : rb;
+  const cuuint64_t ps = b.n_pages > 1 ? (cuuint64_t)b.page_stride * es : rb;
+  cuuint64_t stride[4] = {128, hs, ss, ps};
+  cuuint32_t box[5] = {(cuuint32_t)(ib / es), (cuuint32_t)(rb / ib), 1, (cuuint32_t)rows, 1};
+  cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  *swap = hs > ss;
+  if (*swap) {
+    std::swap(dim[2], dim[3]);
+    std::swap(stride[1], stride[2]);
+    std::swap(box[2], box[3]);
+  }
+  const CUresult r =
+      encode(map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5, pool, dim, stride, box,
+             step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             ib == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : ib == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(Q6W_ERR_ARG, "the pages' strides cannot be described to the copy engine (%d)", (int)r);
+  return Q6W_OK;
+}
+
 template <int HDF, typename KT>
-static int32_t launch(const DecodeArgs& a, cudaStream_t st) {
+static int32_t launch(DecodeArgs a, cudaStream_t st) {
   using S = DecodeShape<HDF, KT>;
   auto kern = decode_kernel<HDF, KT>;
-  constexpr int smem = kDecodeWarps * S::RING;
+  constexpr int smem = 1024 + kDecodeWarps * S::RING;
   static std::mutex mu;
   static bool granted[64] = {false};  // per device
   int dev = 0;
@@ -745,10 +843,17 @@ static int32_t launch(const DecodeArgs& a, cudaStream_t st) {
       granted[dev & 63] = true;
     }
   }
+  DecodeMaps maps;
+  const int rows = std::min(kTile, 1 << a.b.shift);
+  bool swap = false;
+  int32_t rc = pool_map(a.b, a.b.k, a.hd, S::ES, a.F, rows, &maps.k, &swap);
+  if (!rc) rc = pool_map(a.b, a.b.v, a.hd, S::ES, a.F, rows, &maps.v, &swap);
+  if (rc) return rc;
+  a.swap = swap;
   const int64_t most = (int64_t)a.b.n * (a.b.kv_heads / a.F) * a.HB *
-                       std::max<int64_t>(1, (a.b.max_len + kTile - 1) / kTile);
+                       std::max<int64_t>(1, ((int64_t)a.b.max_len + S::KU - 1) / S::KU);
   const int grid = (int)std::min<int64_t>((int64_t)sm_count() * S::CTAS, most);
-  kern<<<grid, kDecodeThreads, smem, st>>>(a);
+  kern<<<grid, kDecodeThreads, smem, st>>>(a, maps);
   Q6W_LAUNCH_CHECK("decode_kernel");
   merge_kernel<<<dim3(grid, std::min(8, a.F > 1 ? a.F * a.b.rep : a.per)), 128, 0, st>>>(a);
   Q6W_LAUNCH_CHECK("merge_kernel");
@@ -765,7 +870,7 @@ int32_t decode_attention(const DecodeArgs& args, bool half, cudaStream_t st) {
   a.per = (a.b.rep + a.HB - 1) / a.HB;
   // narrow heads side by side: while F head_dim <= 64 and F rep <= 8 heads
   a.F = 1;
-  if (a.b.head_stride == a.hd)
+  if (a.b.head_stride == a.hd || a.b.kv_heads == 1)
     while (2 * a.F * a.hd <= 64 && 2 * a.F * a.b.rep <= 8 && a.b.kv_heads % (2 * a.F) == 0) a.F *= 2;
   switch (a.F * a.hd) {
     case 16: return half ? launch<16, __half>(a, st) : launch<16, float>(a, st);
