@@ -343,9 +343,13 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     const uint32_t ring = ((smem_u32(smem_raw) + 1023) & ~1023u) + warp * S::RING;
     const uint8_t* ring_g = smem_raw + (ring - smem_u32(smem_raw));
     Cursor<S::KU> p = cur;
-    const int boxes = b.shift >= 4 ? 1 : kTile >> b.shift;  // boxes of a tile
+    const int bshift = b.shift >= 4 ? 0 : 4 - b.shift;  // 2^bshift boxes of a tile
+    const uint32_t box_bytes = S::TILE >> bshift;
+    const int bt = lane >> bshift, bi = lane & ((1 << bshift) - 1);  // this lane starts box bi of tile bt
+    const int bkey = bt * kTile + (bi << b.shift);
     const int slot_mask = (1 << b.shift) - 1;
     const int32_t* row = b.table;
+    int pblk = 0;
     int pt = 0, pbase = 0, plast = -1, ids = -1;  // page ids: lane i holds the id of page pbase + i
     int istage = 0;
     uint32_t bad = 0;  // bits 2 stage + tile: the tile has a page id out of range
@@ -353,39 +357,39 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       while (p.x < p.x1 && p.key0 >= p.key1) p.next(b, KVB);
       if (p.x >= p.x1) return;
       pt = p.key0;
+      pblk = p.block / a.HB;
       row = b.table + p.s * b.table_stride;
       pbase = p.key0 >> b.shift;
       plast = (p.key1 - 1) >> b.shift;
       ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
     };
-    // Start the next half unit's copies.  Lane t boxes + i starts box i of tile t.
+    // Start the next half unit's copies.
     auto issue = [&](bool values) {
       if (p.x < p.x1) {
-        const int t = lane / boxes, i = lane - t * boxes;
-        const int first = pt + t * kTile + (i << b.shift);  // the box's first key
-        // (a unit's pages are the lanes' or the next 32: both are aligned to the unit)
+        const int first = pt + bkey;  // the box's first key
+        // (a unit's pages are among the lanes' or the next 32: both are aligned to the unit)
         if (!values && ((min(pt + S::KU, p.key1) - 1) >> b.shift) >= pbase + 32) {
           pbase = pt >> b.shift;
           ids = pbase + lane <= plast ? __ldg(row + pbase + lane) : -1;
         }
         const int id = __shfl_sync(kAll, ids, ((first >> b.shift) - pbase) & 31);
-        const bool in = t < NT && first < p.key1, ok = (unsigned)id < (unsigned)b.n_pages;
-        const int count = __popc(__ballot_sync(kAll, in && ok));
+        const bool in = bt < NT && first < p.key1, ok = in && (unsigned)id < (unsigned)b.n_pages;
+        const unsigned good = __ballot_sync(kAll, ok);
         if (!values) {
-          const unsigned wrong = __ballot_sync(kAll, in && !ok);
+          const unsigned wrong = __ballot_sync(kAll, in) & ~good;
           bad &= ~(3u << (2 * istage));
           if (wrong) {
-            const uint32_t one = (1u << boxes) - 1u;
-            bad |= ((wrong & one ? 1u : 0u) | (NT == 2 && (wrong >> boxes) & one ? 2u : 0u)) << (2 * istage);
+            const uint32_t one = (1u << (1 << bshift)) - 1u;
+            bad |= ((wrong & one ? 1u : 0u) | (NT == 2 && (wrong >> (1 << bshift)) & one ? 2u : 0u)) << (2 * istage);
             if (lane == 0) flag(b.status, kErrInput);
           }
         }
-        if (lane == 0) mbar_expect_tx(bar + istage, count * (S::TILE / boxes));
+        if (lane == 0) mbar_expect_tx(bar + istage, __popc(good) * box_bytes);
         __syncwarp();
-        if (in && ok) {
-          const int blk = p.block / a.HB, slot = first & slot_mask;
-          load_box(ring + istage * S::HALF + t * S::TILE + i * (S::TILE / boxes), values ? &maps.v : &maps.k,
-                   a.swap ? slot : blk, a.swap ? blk : slot, id, bar + istage);
+        if (ok) {
+          const int slot = first & slot_mask;
+          load_box(ring + istage * S::HALF + bt * S::TILE + bi * box_bytes, values ? &maps.v : &maps.k,
+                   a.swap ? slot : pblk, a.swap ? pblk : slot, id, bar + istage);
         }
         if (values) {
           pt += S::KU;
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     // Wait for the oldest half unit, and start the load that takes the place of
     // the one before it (which every lane has read), STG - 1 halves ahead.
     auto advance = [&](bool values) {
-      if (!mbar_wait(bar + stage, phase)) late = true;
+      if (!mbar_try_wait(bar + stage, phase) && !mbar_wait(bar + stage, phase)) late = true;
       __syncwarp();
       issue(values != ((STG - 1) % 2 != 0));
       const uint8_t* at = ring_g + stage * S::HALF;
@@ -728,48 +732,66 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
 }
 
 // Joins the pieces of the items that several CTAs hold: block (c, r) takes
-// head r of the item that starts in CTA c.  The weights of the pieces are
-// found by all threads, then the threads share the pieces out: 128 / head_dim
-// (at least one) groups of a head's dims.
-__global__ void __launch_bounds__(128) merge_kernel(DecodeArgs a) {
+// head r of the item that starts in CTA c.  All threads find the pieces'
+// weights, then groups of head_dim / 4 threads share the pieces out.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeMost = 1024;  // pieces of an item: the CTAs of a grid
+
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
   const int4 d = a.desc[blockIdx.x];
   if (d.z == 0) return;
   int h0, nr;
   block_heads(a, d.y, h0, nr);
   const int r = blockIdx.y;
   if (r >= nr) return;
-  __shared__ float red[4], so[128];
+  __shared__ float red[2][kMergeThreads / 32], w[kMergeMost];
+  __shared__ float4 so[kMergeThreads];
   const int STATE = state_floats(a.hd), hd = a.hd, M0 = 8 * hd + r, L0 = 8 * hd + 8 + r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto piece = [&](int k) { return a.part + ((size_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * STATE; };
+  // (the first CTA's piece is its second slot)
+  const float* base = a.part + (size_t)blockIdx.x * 2 * STATE;
+  auto piece = [&](int k) { return base + ((size_t)k * 2 + (k == 0 ? 1 : 0)) * STATE; };
   float M = -INFINITY;
-  for (int k = tid; k < d.z; k += 128) M = fmaxf(M, piece(k)[M0]);
+  for (int k = tid; k < d.z; k += kMergeThreads) {
+    w[k] = piece(k)[M0];
+    M = fmaxf(M, w[k]);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) red[warp] = M;
+  if (lane == 0) red[0][warp] = M;
   __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int i = 0; i < kMergeThreads / 32; ++i) M = fmaxf(M, red[0][i]);
   const float ref = ref_of(M);
-  const int groups = 128 / hd, x = tid % hd, grp = tid / hd;
-  float o = 0.f, l = 0.f;
-#pragma unroll 8
+  float l = 0.f;
+  for (int k = tid; k < d.z; k += kMergeThreads) {
+    w[k] = ex2(w[k] - ref);
+    l += w[k] * piece(k)[L0];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  const int per = hd / 4, groups = kMergeThreads / per, x = tid % per, grp = tid / per;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
   for (int k = grp; k < d.z; k += groups) {
-    const float* p = piece(k);
-    const float w = ex2(p[M0] - ref);
-    o += w * p[r * hd + x];
-    l += w * p[L0];
+    const float4 v = *reinterpret_cast<const float4*>(piece(k) + r * hd + 4 * x);
+    o.x = fmaf(w[k], v.x, o.x);
+    o.y = fmaf(w[k], v.y, o.y);
+    o.z = fmaf(w[k], v.z, o.z);
+    o.w = fmaf(w[k], v.w, o.w);
   }
   so[tid] = o;
   __syncthreads();
   if (tid < hd) {
-    for (int k = 1; k < groups; ++k) o += so[tid + k * hd];
-  }
-  __syncthreads();
-  so[tid] = l;
-  __syncthreads();
-  if (tid < hd) {
-    for (int k = 1; k < groups; ++k) l += so[tid + k * hd];
-    a.out[((int64_t)d.x * a.H + h0 + r) * hd + x] = l == 0.f ? 0.f : o / l;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; ++i) l += red[1][i];
+    const float* col = reinterpret_cast<const float*>(so) + tid;
+    float sum = 0.f;
+    for (int k = 0; k < groups; ++k) sum += col[k * hd];
+    a.out[((int64_t)d.x * a.H + h0 + r) * hd + tid] = l == 0.f ? 0.f : sum / l;
   }
 }
 
@@ -852,10 +874,10 @@ static int32_t launch(DecodeArgs a, cudaStream_t st) {
   a.swap = swap;
   const int64_t most = (int64_t)a.b.n * (a.b.kv_heads / a.F) * a.HB *
                        std::max<int64_t>(1, ((int64_t)a.b.max_len + S::KU - 1) / S::KU);
-  const int grid = (int)std::min<int64_t>((int64_t)sm_count() * S::CTAS, most);
+  const int grid = (int)std::min<int64_t>(std::min(sm_count() * S::CTAS, kMergeMost), most);
   kern<<<grid, kDecodeThreads, smem, st>>>(a, maps);
   Q6W_LAUNCH_CHECK("decode_kernel");
-  merge_kernel<<<dim3(grid, std::min(8, a.F > 1 ? a.F * a.b.rep : a.per)), 128, 0, st>>>(a);
+  merge_kernel<<<dim3(grid, std::min(8, a.F > 1 ? a.F * a.b.rep : a.per)), kMergeThreads, 0, st>>>(a);
   Q6W_LAUNCH_CHECK("merge_kernel");
   return Q6W_OK;
 }
