@@ -14,7 +14,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = ["csrc/codec.cu", "csrc/linear.cu", "csrc/model.cu", "csrc/paged.cu", "csrc/paged_decode.cu"]
+SOURCES = ["csrc/codec.cu", "csrc/linear.cu", "csrc/model.cu", "csrc/paged.cu", "csrc/paged_decode.cu", "csrc/paged_tc.cu"]
 OUT = HERE / "q6w_b200" / "libq6w_b200.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -101,111 +101,6 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   }
 }
 
-// ---- attention -----------------------------------------------------------------
-
-struct AttnArgs {
-  Batch b;
-  const float* q;
-  int64_t ldq;
-  float* out;
-  int32_t H, zero;
-  const int32_t* prefix_pages;
-  int32_t prefix_len;
-  float scale;  // log2(e) / sqrt(head_dim)
-};
-
-template <int HD>
-__device__ __forceinline__ float key_dot(const float* q, const float* k) {
-  float d = 0.f;
-#pragma unroll
-  for (int i = 0; i < HD; i += 4) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(k + i));
-    d = fmaf(q[i], x.x, d);
-    d = fmaf(q[i + 1], x.y, d);
-    d = fmaf(q[i + 2], x.z, d);
-    d = fmaf(q[i + 3], x.w, d);
-  }
-  return d;
-}
-template <int HD>
-__device__ __forceinline__ float key_dot(const float* q, const __half* k) {
-  float d = 0.f;
-#pragma unroll
-  for (int i = 0; i < HD; i += 2) {
-    const float2 x = __half22float2(__ldg(reinterpret_cast<const __half2*>(k + i)));
-    d = fmaf(q[i], x.x, d);
-    d = fmaf(q[i + 1], x.y, d);
-  }
-  return d;
-}
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-
-// One warp per (token, query head); a lane takes every 32nd visible key with
-// a running maximum and sum of its own, the lanes' states joined at the end.
-template <int HD, typename KT>
-__global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
-  __shared__ float qs[4][HD];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t item = (int64_t)blockIdx.x * 4 + warp;
-  if (item >= (int64_t)a.b.T * a.H) return;
-  const int t = (int)(item / a.H), h = (int)(item % a.H), g = h / a.b.rep;
-  float* out = a.out + item * HD;
-  const int s = token_seq(a.b, t, lane);
-  if (s < 0 || s >= a.b.n) {
-    if (a.zero)
-      for (int d = lane; d < HD; d += 32) out[d] = 0.f;
-    return;
-  }
-  for (int d = lane; d < HD; d += 32) qs[warp][d] = a.q[t * a.ldq + h * HD + d];
-  __syncwarp();
-  int t0, t1;
-  seq_tokens(a.b, s, t0, t1);
-  const int seen = min(max(seq_length(a.b, s) - (t1 - t) + 1, 0), a.b.max_len);
-  float m = -INFINITY, l = 0.f, acc[HD];
-#pragma unroll
-  for (int d = 0; d < HD; ++d) acc[d] = 0.f;
-  const int P = a.prefix_len;
-  for (int64_t i = lane; i < (int64_t)P + seen; i += 32) {
-    const int at = (int)(i < P ? i : i - P);
-    const int32_t* ids = i < P ? a.prefix_pages : a.b.table + s * a.b.table_stride;
-    const int page = __ldg(ids + (at >> a.b.shift));
-    float sc;
-    const KT* vr = nullptr;
-    if (page < 0 || page >= a.b.n_pages) {
-      flag(a.b.status, kErrInput);
-      sc = NAN;
-    } else {
-      const int64_t off = page * a.b.page_stride + (int64_t)(at & ((1 << a.b.shift) - 1)) * a.b.slot_stride +
-                          g * a.b.head_stride;
-      sc = key_dot<HD>(qs[warp], static_cast<const KT*>(a.b.k) + off) * a.scale;
-      vr = static_cast<const KT*>(a.b.v) + off;
-    }
-    const float mn = fmaxf(m, sc);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float al = exp2f(m - ref), p = exp2f(sc - ref);
-    m = mn;
-    l = l * al + p;
-#pragma unroll
-    for (int d = 0; d < HD; ++d) acc[d] = fmaf(p, vr ? widen(vr[d]) : 0.f, acc[d] * al);
-  }
-  float M = m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float ref = M == -INFINITY ? 0.f : M;
-  const float w = exp2f(m - ref);
-  float L = l * w;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-#pragma unroll
-  for (int d = 0; d < HD; ++d) {
-    float x = acc[d] * w;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (lane == (d & 31)) out[d] = L == 0.f ? 0.f : x / L;
-  }
-}
-
 // ---- host ------------------------------------------------------------------------
 
 static int32_t check_batch(const char* who, const q6w_paged_batch* p, int32_t n_tokens, Batch* b) {
@@ -265,23 +160,54 @@ static int32_t check_heads(const char* who, const q6w_paged_batch* p, int32_t n_
   return Q6W_OK;
 }
 
-template <int HD>
-static void launch_rows(const AttnArgs& a, bool half, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)a.b.T * a.H + 3) / 4);
-  if (half)
-    attn_rows_kernel<HD, __half><<<grid, 128, 0, st>>>(a);
-  else
-    attn_rows_kernel<HD, float><<<grid, 128, 0, st>>>(a);
+// The workspace: a call's regions in order, each 256-byte aligned.  Base null: sizes only.
+struct Space {
+  char* at;
+  size_t used = 0;
+  explicit Space(void* base) : at(static_cast<char*>(base)) {}
+  template <typename T>
+  T* take(size_t count) {
+    T* p = at ? reinterpret_cast<T*>(at + used) : nullptr;
+    used += (count * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+struct Regions {
+  char* decode = nullptr;
+  float *own = nullptr, *own_ml = nullptr, *prefix = nullptr, *prefix_ml = nullptr, *state = nullptr;
+  int4* desc = nullptr;
+  int64_t* line = nullptr;
+};
+
+static size_t layout(const Batch& b, int hd, int H, bool half, int prefix_length, void* base, Regions* r) {
+  Space s(base);
+  if (b.starts) {
+    const size_t rows = rows_own_rows(hd, half);
+    r->own = s.take<float>(rows * hd);
+    r->own_ml = s.take<float>(rows * 2);
+    r->desc = s.take<int4>((size_t)sm_count() * 2);
+    r->line = s.take<int64_t>((size_t)b.n + 1);
+  } else {
+    r->decode = s.take<char>(decode_workspace(hd));
+  }
+  if (prefix_length > 0) {
+    const size_t rows = rows_prefix_rows(b, prefix_length, hd, half);
+    r->prefix = s.take<float>(rows * hd);
+    r->prefix_ml = s.take<float>(rows * 2);
+    r->state = s.take<float>((size_t)b.T * H * 2);
+  }
+  return s.used;
 }
 
 static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_t* prefix_pages, int32_t prefix_length,
                          int32_t n_tokens, int32_t n_heads, const float* queries, int64_t query_stride, float* output,
                          int32_t zero_padding, void* workspace, size_t workspace_bytes, q6w_stream_t stream) {
   clear_error();
-  AttnArgs a;
-  int32_t st = check_batch(who, p, n_tokens, &a.b);
+  Batch b;
+  int32_t st = check_batch(who, p, n_tokens, &b);
   if (st) return st;
-  st = check_heads(who, p, n_heads, &a.b);
+  st = check_heads(who, p, n_heads, &b);
   if (st) return st;
   if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
   if (p->page_size * p->head_dim * (p->kv_dtype == Q6W_KV_F16 ? 2 : 4) < 128)
@@ -292,39 +218,60 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
     return fail(Q6W_ERR_ALIGN, "%s: queries (and their stride) and output must be 16-byte aligned", who);
   if (query_stride < (int64_t)n_heads * p->head_dim)
     return fail(Q6W_ERR_ARG, "%s: query_stride is shorter than a token's heads", who);
-  const size_t need = q6w_paged_workspace_bytes(p, n_tokens, n_heads, prefix_length);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(Q6W_ERR_ARG, "%s: the workspace needs %zu bytes", who, need);
-  a.q = queries;
-  a.ldq = query_stride;
-  a.out = output;
-  a.H = n_heads;
-  a.zero = zero_padding;
-  a.prefix_pages = prefix_pages;
-  a.prefix_len = prefix_length;
-  a.scale = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
+  const int hd = p->head_dim;
   const bool half = p->kv_dtype == Q6W_KV_F16;
+  Regions r;
+  const size_t need = layout(b, hd, n_heads, half, prefix_length, workspace, &r);
+  if (!workspace || workspace_bytes < need)
+    return fail(Q6W_ERR_ARG, "%s: the workspace needs %zu bytes", who, need);
+  if (!aligned(workspace, 256)) return fail(Q6W_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
   cudaStream_t s = (cudaStream_t)stream;
-  if (!p->query_starts && prefix_length == 0) {
-    DecodeArgs d;
-    d.b = a.b;
+  const float scale = (float)(1.4426950408889634 / sqrt((double)hd));
+  if (b.starts && zero_padding) {
+    st = zero_padding_rows(b, output, n_heads * hd, s);
+    if (st) return st;
+  }
+  if (b.n == 0) return Q6W_OK;
+  TcArgs t = {};
+  t.b = b;
+  t.q = queries;
+  t.ldq = query_stride;
+  t.out = output;
+  t.state = r.state;
+  t.desc = r.desc;
+  t.line = r.line;
+  t.H = n_heads;
+  t.scale = scale;
+  t.prefix_len = prefix_length;
+  TcArgs pre = t;
+  pre.part = r.prefix;
+  pre.part_ml = r.prefix_ml;
+  pre.b.table = prefix_pages;
+  pre.b.starts = nullptr;
+  if (prefix_length > 0) {
+    st = rows_prefix(pre, hd, half, s);
+    if (st) return st;
+  }
+  if (b.starts) {
+    t.part = r.own;
+    t.part_ml = r.own_ml;
+    st = rows_own(t, hd, half, s);
+  } else {
+    DecodeArgs d = {};
+    d.b = b;
     d.q = queries;
     d.ldq = query_stride;
     d.out = output;
+    d.state = r.state;
     d.H = n_heads;
-    d.hd = p->head_dim;
-    d.scale = a.scale;
-    d.desc = static_cast<int4*>(workspace);
-    return decode_attention(d, half, s);
+    d.hd = hd;
+    d.scale = scale;
+    d.desc = reinterpret_cast<int4*>(r.decode);
+    st = decode_attention(d, half, s);
   }
-  switch (p->head_dim) {
-    case 16: launch_rows<16>(a, half, s); break;
-    case 32: launch_rows<32>(a, half, s); break;
-    case 64: launch_rows<64>(a, half, s); break;
-    default: launch_rows<128>(a, half, s); break;
-  }
-  Q6W_LAUNCH_CHECK("attn_rows_kernel");
-  return Q6W_OK;
+  if (st || prefix_length == 0) return st;
+  pre.own_rows = b.starts;
+  return rows_join(pre, hd, half, s);
 }
 
 }  // namespace paged
@@ -387,9 +334,11 @@ extern "C" size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_
                                             int32_t prefix_length) {
   paged::Batch b;
   if (paged::check_batch("q6w_paged_workspace_bytes", batch, n_tokens, &b) ||
-      paged::check_heads("q6w_paged_workspace_bytes", batch, n_heads, &b) || prefix_length < 0)
+      paged::check_heads("q6w_paged_workspace_bytes", batch, n_heads, &b) || prefix_length < 0 ||
+      prefix_length > (1 << 30))
     return 0;
-  return batch->query_starts || prefix_length ? 0 : paged::decode_workspace(batch->head_dim);
+  paged::Regions r;
+  return paged::layout(b, batch->head_dim, n_heads, batch->kv_dtype == Q6W_KV_F16, prefix_length, nullptr, &r);
 }
 
 extern "C" int32_t q6w_paged_attention(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,

@@ -6,6 +6,8 @@
 // heads have strides of their own.
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 
 #include "async.cuh"
@@ -73,6 +75,23 @@ __device__ __forceinline__ int token_seq(const Batch& b, int t, int lane) {
   return lo - 1;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
+__device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ int64_t owner_of(int64_t unit, int64_t units, int64_t workers) {
+  // worker w holds units [w units / workers, (w + 1) units / workers)
+  return ((unit + 1) * workers + units - 1) / units - 1;
+}
+
+// The pool's tensor map (paged_decode.cu).
+int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, int segments, CUtensorMap* map,
+                 bool* swap);
+
 // ---- decode attention (paged_decode.cu) -------------------------------------
 
 struct DecodeArgs {
@@ -80,6 +99,7 @@ struct DecodeArgs {
   const float* q;
   int64_t ldq;
   float* out;
+  float* state;     // [row][m, l], or null; with it `out` takes the unnormalised outputs
   float* wpart;     // [warp of the grid][2][state]: pieces of items
   float* part;      // [CTA][2][state]: pieces joined inside a CTA
   int4* desc;       // [CTA]: item that starts in the CTA and goes on: {s, block, CTAs, 0}
@@ -92,6 +112,35 @@ struct DecodeArgs {
 // One query token a sequence; workspace (desc): decode_workspace bytes.
 int32_t decode_attention(const DecodeArgs& a, bool half, cudaStream_t st);
 size_t decode_workspace(int head_dim);
+
+// ---- many rows over the same keys (paged_tc.cu) --------------------------------
+
+struct TcArgs {
+  Batch b;
+  const float* q;
+  int64_t ldq;
+  float* out;
+  float* state;      // [row][m, l], or null; with it `out` takes the unnormalised outputs
+  float* part;       // pieces: outputs [..][head_dim]; own rows [CTA][2][block row], prefix [piece][item][block row]
+  float* part_ml;    // pieces: [..][m, l]
+  int4* desc;        // [CTA][2]: block that starts in the CTA and goes on: {first token, kv head, block, CTAs}, {rows}
+  int64_t* line;     // [n + 1]: units of the sequences in front, one kv head's
+  const int32_t* own_rows;  // the ragged batch's query_starts (prefix join), or null
+  int32_t H, swap;
+  int32_t prefix, prefix_len, items;  // over the prefix (its pages in b.table), blocks of all kv heads
+  float scale;       // log2(e) / sqrt(head_dim)
+};
+
+struct TcMaps {
+  CUtensorMap k, v;
+};
+
+int32_t rows_own(const TcArgs& a, int hd, bool half, cudaStream_t st);
+int32_t rows_prefix(const TcArgs& a, int hd, bool half, cudaStream_t st);
+int32_t rows_join(const TcArgs& a, int hd, bool half, cudaStream_t st);
+size_t rows_own_rows(int hd, bool half);  // piece rows that rows_own / rows_prefix need
+size_t rows_prefix_rows(const Batch& b, int prefix_len, int hd, bool half);
+int32_t zero_padding_rows(const Batch& b, float* out, int row, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace q6w

@@ -119,19 +119,6 @@ struct DecodeMaps {
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
-__device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
-
-__device__ __forceinline__ int64_t owner_of(int64_t unit, int64_t units, int64_t workers) {
-  // worker w holds units [w units / workers, (w + 1) units / workers)
-  return ((unit + 1) * workers + units - 1) / units - 1;
-}
-
 // The line of units: prefix sums over 256 stretches of sequences.
 struct Line {
   int64_t pref[kDecodeThreads];
@@ -647,7 +634,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       for (int hh = 0; hh < 2; ++hh) {
         const int n = 2 * c + hh;
         const float l = hh ? l1 : l0;
-        const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        const float inv = !whole || a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
         const int f = a.F > 1 ? n / b.rep : 0;
         float* dst = whole ? a.out + ((int64_t)s * a.H + h0 + n) * a.hd : slot + n * a.hd;
         if (n < nr) {
@@ -662,9 +649,14 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
             }
           }
         }
-        if (!whole && g == 0) {
-          slot[8 * a.hd + n] = (hh ? lim1 : lim0) == -INFINITY ? -INFINITY : (hh ? ref1 : ref0);
-          slot[8 * a.hd + 8 + n] = l;
+        if ((!whole || a.state) && g == 0) {
+          const float m = (hh ? lim1 : lim0) == -INFINITY ? -INFINITY : (hh ? ref1 : ref0);
+          if (!whole) {
+            slot[8 * a.hd + n] = m;
+            slot[8 * a.hd + 8 + n] = l;
+          } else if (n < nr) {
+            *reinterpret_cast<float2*>(a.state + ((int64_t)s * a.H + h0 + n) * 2) = make_float2(m, l);
+          }
         }
       }
       if (lane == 0 && !whole) segs[2 * warp + which] = {cur.first, s, cur.block, 1, begin, end};
@@ -711,7 +703,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           l += w * p[L0 + r];
         }
       if (f.begin && end) {
-        a.out[((int64_t)f.s * a.H + h0) * hd + x] = l == 0.f ? 0.f : o / l;
+        const int64_t row = (int64_t)f.s * a.H + h0;
+        a.out[row * hd + x] = a.state ? o : (l == 0.f ? 0.f : o / l);
+        if (a.state && x % hd == 0) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(M, l);
       } else {
         dst[x] = o;
         if (x % hd == 0) {
@@ -791,7 +785,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
     const float* col = reinterpret_cast<const float*>(so) + tid;
     float sum = 0.f;
     for (int k = 0; k < groups; ++k) sum += col[k * hd];
-    a.out[((int64_t)d.x * a.H + h0 + r) * hd + tid] = l == 0.f ? 0.f : sum / l;
+    const int64_t row = (int64_t)d.x * a.H + h0 + r;
+    a.out[row * hd + tid] = a.state ? sum : (l == 0.f ? 0.f : sum / l);
+    if (a.state && tid == 0) *reinterpret_cast<float2*>(a.state + row * 2) = make_float2(M, l);
   }
 }
 
@@ -818,9 +814,10 @@ static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
 }
 
 // The pool as (ib bytes, segments, kv-head blocks, slots, pages) -- blocks and
-// slots in ascending order of their strides -- with a box of `rows` slots of
-// one block.
-int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, CUtensorMap* map, bool* swap) {
+// slots in ascending order of their strides -- with a box of `rows` slots and
+// `segments` segments of one block.
+int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, int segments, CUtensorMap* map,
+                 bool* swap) {
   auto encode = map_encoder();
   if (!encode) return fail(Q6W_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const int rb = F * hd * es, ib = rb < 128 ? rb : 128;
@@ -832,7 +829,7 @@ int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, CU
   const cuuint64_t hs = b.kv_heads / F > 1 ? (cuuint64_t)F * b.head_stride * es : rb;
   const cuuint64_t ps = b.n_pages > 1 ? (cuuint64_t)b.page_stride * es : rb;
   cuuint64_t stride[4] = {128, hs, ss, ps};
-  cuuint32_t box[5] = {(cuuint32_t)(ib / es), (cuuint32_t)(rb / ib), 1, (cuuint32_t)rows, 1};
+  cuuint32_t box[5] = {(cuuint32_t)(ib / es), (cuuint32_t)segments, 1, (cuuint32_t)rows, 1};
   cuuint32_t step[5] = {1, 1, 1, 1, 1};
   *swap = hs > ss;
   if (*swap) {
@@ -868,8 +865,8 @@ static int32_t launch(DecodeArgs a, cudaStream_t st) {
   DecodeMaps maps;
   const int rows = std::min(kTile, 1 << a.b.shift);
   bool swap = false;
-  int32_t rc = pool_map(a.b, a.b.k, a.hd, S::ES, a.F, rows, &maps.k, &swap);
-  if (!rc) rc = pool_map(a.b, a.b.v, a.hd, S::ES, a.F, rows, &maps.v, &swap);
+  int32_t rc = pool_map(a.b, a.b.k, a.hd, S::ES, a.F, rows, S::RB / S::IB, &maps.k, &swap);
+  if (!rc) rc = pool_map(a.b, a.b.v, a.hd, S::ES, a.F, rows, S::RB / S::IB, &maps.v, &swap);
   if (rc) return rc;
   a.swap = swap;
   const int64_t most = (int64_t)a.b.n * (a.b.kv_heads / a.F) * a.HB *

@@ -1,0 +1,1059 @@
+// Attention of many query rows over the same paged keys, on tcgen05: prompts
+// and chunks of prompts (causal), and a batch over its shared prefix.
+//
+// Mathematics.  The rows that share a kv head's keys are the query tokens times
+// the `rep` heads of the group: row = token rep + r.  A CTA holds a block of
+// 128 (256) rows and walks over its keys in units of 128 (FP16 pages) or 64
+// (FP32): S = Q K^T, p = 2^(c s - m) with a reference m a row that moves only
+// when a score passes it by more than 8, l += p, O += P V.  Pieces of a
+// block's keys join as in the decode kernel.
+//
+// Operands.  FP16 pages: K and V enter as they are, Q (scaled by a power of
+// two a row) and P as FP16 hi + lo, 22 bits: 2 + 2 MMAs.  FP32 pages: every
+// operand enters as three BF16 parts (24 bits) and the products down to
+// 2^-16 are kept, 6 + 6 MMAs, the small ones first.  Q and P are the MMA's A
+// operand and live in tensor memory, where the softmax threads (one row each:
+// TMEM lane = row) write them; P overlays the S that it was made from.  K is
+// the K-major and V the MN-major B operand, both rows of keys as they lie in
+// the pages, so nothing is transposed.
+//
+// Sums.  The MMA's FP32 accumulator loses up to a unit in the last place with
+// every added product (the sum is cut, not rounded), so O stays in it for kFlush
+// units only and is then added to the row's registers, rounded to nearest.
+//
+// Bound.  Per unit and 128 rows: 2 (12) x 128 x keys x head_dim x 2 MMA flop, 128
+// x keys exponentials and about ten FP32 instructions a score; with two row
+// tiles in a CTA (head_dim <= 64) the softmax of one runs under the MMAs of the
+// other, with one tile (head_dim 128) S has two buffers.
+//
+// Roles: warps 0-3 (4-7) softmax of a tile, then four load warps, one MMA warp.
+// Load warps fetch FP16 units by TMA boxes; FP32 units, units with a bad page
+// id and units that some row does not see whole go through registers: keys no
+// row sees become zeros, and a key whose value is not finite becomes a NaN key
+// with zero values, so that only the rows that see it become NaN.
+//
+// Blocks' units lie on one line; every CTA takes an equal stretch (as the
+// decode kernel's warps do).  Every wait is bounded; a timeout sets the status
+// bit and makes the CTA stop.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <string.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace q6w {
+namespace paged {
+
+constexpr int kTcMaxStages = 4;
+
+template <int HD, typename KT>
+struct TcShape {
+  static constexpr bool kHalf = std::is_same<KT, __half>::value;
+  static constexpr int TILES = HD <= 64 ? 2 : 1;   // row tiles of a CTA
+  static constexpr int BUFS = 3 - TILES;           // S buffers of a tile
+  static constexpr int ROWS = 128 * TILES;
+  static constexpr int KEYS = kHalf ? 128 : 64;
+  static constexpr int QP = kHalf ? 2 : 3;         // parts of Q and P
+  static constexpr int KP = kHalf ? 1 : 3;         // parts of K and V
+  static constexpr int RB = HD * 2 < 128 ? HD * 2 : 128;  // bytes of a panel row = swizzle span
+  static constexpr int PANELS = HD * 2 / RB;
+  static constexpr int PANEL = KEYS * RB;
+  static constexpr int PART = PANEL * PANELS;      // bytes of a unit's keys (or values), one part
+  static constexpr int HALF = KP * PART;
+  static constexpr int STG = 192 * 1024 / (2 * HALF) < kTcMaxStages ? 192 * 1024 / (2 * HALF) : kTcMaxStages;
+  // tensor memory columns of a tile: Q parts, S / P buffers, O
+  static constexpr int QC = (QP * HD / 2 + 31) / 32 * 32;
+  static constexpr int SC = kHalf ? KEYS : 96;     // P: QP x KEYS / 2 columns over S
+  static constexpr int S0 = kHalf ? 0 : 32;        // S inside its buffer (P's first chunk stays in front of unread S)
+  static constexpr int TC = QC + BUFS * SC + (HD < 32 ? 32 : HD);
+  static_assert(TC * TILES <= 512, "tensor memory columns");
+  static constexpr int SOFT = 4 * TILES;           // softmax warps
+  // Softmax, load and MMA warps in groups of four with registers of their own
+  // (what the block was launched with, 64 K / THREADS a thread, divided anew).
+  static constexpr int THREADS = 32 * (SOFT + 8);
+  static constexpr int REGS = TILES == 2 ? 128 : 168;
+  static constexpr int SOFT_REGS = TILES == 2 ? 168 : 240, LOAD_REGS = TILES == 2 ? 104 : 160, MMA_REGS = TILES == 2 ? 72 : 104;
+  static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
+  static constexpr int kFlush = 4;
+  static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
+};
+
+// One MMA shared-memory descriptor: rows of RB bytes swizzled over RB, eight-row
+// groups `group` bytes apart.  (K-major: the groups are along the keys, the MMA's
+// N; MN-major: along the keys too, its K; both offsets are given the same
+// stride, as the other one is not used by operands one swizzle span wide.)
+template <int RB>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+  constexpr uint64_t layout = RB == 128 ? 2 : RB == 64 ? 4 : 6;
+  constexpr uint64_t group = RB * 8 / 16;
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (group << 16) | (group << 32) | (1ull << 46) | (layout << 61);
+}
+
+// Byte place of byte `at` of row `row` in a swizzled panel.
+template <int RB>
+__device__ __forceinline__ int panel_place(int row, int at) {
+  const int x = row * RB + at;
+  return RB == 128 ? x ^ ((x >> 3) & 0x70) : RB == 64 ? x ^ ((x >> 3) & 0x30) : x ^ ((x >> 3) & 0x10);
+}
+
+// 32 (16) consecutive FP32 columns of this thread's TMEM lane.  The wait names the
+// destination registers, so no use of them is scheduled before it.
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+
+// A thread's registers from here on (a whole group of four warps calls it).
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// The AND of `ok` over the four load warps (all of them call it).
+__device__ __forceinline__ bool load_warps_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.aligned.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
+}
+
+// Two values -> packed parts, first value in the low half.
+template <bool HALF_PARTS, int N>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (HALF_PARTS) {
+      const __half2 h = __floats2half2_rn(x, y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (i + 1 < N) {
+        const float2 f = __half22float2(h);
+        x -= f.x;
+        y -= f.y;
+      }
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (i + 1 < N) {
+        x -= __uint_as_float(w[i] << 16);
+        y -= __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+// ---- the line of units -----------------------------------------------------------
+
+// A block of rows of one (sequence, kv head) and a stretch [u0, u1) of its units.
+struct Piece {
+  int64_t x;              // the line's unit at u0
+  int s, kv, j;           // sequence, kv head, row block
+  int tok0, count, past;  // first query token and tokens of the sequence, cached tokens in front of them
+  int keys, units;        // keys that the block's last row sees, units of the block
+  int u0, u1;
+};
+
+template <int ROWS, int KEYS>
+struct Walk {
+  const TcArgs& a;
+  Piece p;
+  int64_t end;
+  __device__ Walk(const TcArgs& args) : a(args) {}
+  __device__ __forceinline__ int rep() const { return a.b.rep; }
+  __device__ __forceinline__ int seen(int tok) const {  // keys that token tok (0 .. count-1) sees
+    return a.prefix ? a.prefix_len : min(max(p.past + tok + 1, 0), a.b.max_len);
+  }
+  __device__ __forceinline__ int rows() const { return min(ROWS, p.count * rep() - p.j * ROWS); }
+  __device__ void sequence() {
+    if (a.prefix) {
+      p.tok0 = 0;
+      p.count = a.b.T;
+      p.past = 0;
+    } else {
+      int t1;
+      seq_tokens(a.b, p.s, p.tok0, t1);
+      p.count = t1 - p.tok0;
+      p.past = max(__ldg(a.b.lengths + p.s), 0) - p.count;
+    }
+  }
+  __device__ void block() {
+    p.keys = seen((p.j * ROWS + rows() - 1) / rep());
+    p.units = max(1, (p.keys + KEYS - 1) / KEYS);
+  }
+  __device__ int blocks() const { return (p.count * rep() + ROWS - 1) / ROWS; }
+  __device__ void begin(int64_t x, int64_t x1) {
+    p.x = x;
+    end = x1;
+    if (x >= x1) return;
+    int64_t rem = x;
+    p.s = 0;
+    if (a.prefix) {
+      sequence();
+      const int per = max(1, (a.prefix_len + KEYS - 1) / KEYS), nb = blocks();
+      p.kv = (int)(rem / ((int64_t)per * nb));
+      rem -= (int64_t)p.kv * per * nb;
+      p.j = (int)(rem / per);
+      rem -= (int64_t)p.j * per;
+      block();
+    } else {
+      int lo = 0, hi = a.b.n;  // line[lo] kv_heads <= x < line[hi] kv_heads
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.line[mid] * a.b.kv_heads <= x) lo = mid; else hi = mid;
+      }
+      p.s = lo;
+      rem -= a.line[lo] * a.b.kv_heads;
+      sequence();
+      const int64_t per = a.line[lo + 1] - a.line[lo];
+      p.kv = (int)(rem / per);
+      rem -= p.kv * per;
+      for (p.j = 0;; ++p.j) {
+        block();
+        if (rem < p.units) break;
+        rem -= p.units;
+      }
+    }
+    p.u0 = (int)rem;
+    p.u1 = (int)min((int64_t)p.units, rem + (x1 - x));
+  }
+  __device__ __forceinline__ bool more() const { return p.x < end; }
+  __device__ void next() {
+    p.x += p.u1 - p.u0;
+    if (p.x >= end) return;
+    if (++p.j >= blocks()) {
+      p.j = 0;
+      if (++p.kv == a.b.kv_heads) {
+        p.kv = 0;
+        do {
+          ++p.s;
+          sequence();
+        } while (p.count == 0);
+      }
+    }
+    block();
+    p.u0 = 0;
+    p.u1 = (int)min((int64_t)p.units, end - p.x);
+  }
+};
+
+// Prefix sums of the sequences' units of one kv head, line[0 .. n].
+template <int ROWS, int KEYS>
+__global__ void __launch_bounds__(1024) line_kernel(TcArgs a, int64_t* line) {
+  __shared__ int64_t part[32];
+  __shared__ int64_t carry;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    carry = 0;
+    line[0] = 0;
+  }
+  Walk<ROWS, KEYS> w(a);
+  for (int base = 0; base < a.b.n; base += 1024) {
+    __syncthreads();
+    const int s = base + tid;
+    int64_t u = 0;
+    if (s < a.b.n) {
+      if (__ldg(a.b.lengths + s) > a.b.max_len) flag(a.b.status, kErrInput);
+      w.p.s = s;
+      w.sequence();
+      const int nb = w.blocks();
+      for (w.p.j = 0; w.p.j < nb; ++w.p.j) {
+        w.block();
+        u += w.p.units;
+      }
+    }
+    int64_t incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    int64_t before = carry, total = 0;
+    for (int i = 0; i < 32; ++i) {
+      if (i < warp) before += part[i];
+      total += part[i];
+    }
+    if (s < a.b.n) line[s + 1] = before + incl;
+    __syncthreads();
+    if (tid == 0) carry += total;
+  }
+}
+
+// ---- the kernel ----------------------------------------------------------------------
+
+template <int HD, typename KT>
+__global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
+    rows_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
+  using S = TcShape<HD, KT>;
+  constexpr bool kHalf = S::kHalf;
+  constexpr int KEYS = S::KEYS, STG = S::STG, TILES = S::TILES, BUFS = S::BUFS, QP = S::QP, RB = S::RB;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t k_full[STG], k_empty[STG], v_full[STG], v_empty[STG];
+  __shared__ uint64_t q_full[TILES], s_full[2], p_full[2], pv_done[TILES], drain;
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int stop;
+  __shared__ uint32_t odd_keys[4];  // keys of the unit whose values are not finite
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  if (warp == S::SOFT + 4) {
+    tc::tmem_alloc(&tmem_base, 512);
+    tc::tmem_relinquish();
+  }
+  if (tid == 0) {
+    if (!a.prefix) a.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    for (int i = 0; i < STG; ++i) {
+      mbar_init(k_full + i, 4);
+      mbar_init(v_full + i, 4);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_empty + i, 1);
+    }
+    for (int i = 0; i < TILES; ++i) {
+      mbar_init(q_full + i, 4);
+      mbar_init(pv_done + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+    }
+    mbar_init(&drain, 1);
+    stop = 0;
+    fence_mbar_init();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  const int64_t units = a.prefix
+                            ? (int64_t)a.b.kv_heads * ((a.b.T * a.b.rep + S::ROWS - 1) / S::ROWS) *
+                                  max(1, (a.prefix_len + KEYS - 1) / KEYS)
+                            : a.line[a.b.n] * a.b.kv_heads;
+  const int64_t workers = min((int64_t)gridDim.x, units);
+  const int64_t c = blockIdx.x;
+  Walk<S::ROWS, KEYS> w(a);
+  if (c < workers)
+    w.begin(c * units / workers, (c + 1) * units / workers);
+  else
+    w.begin(0, 0);
+  const int64_t x0 = w.p.x;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (stop) return false;
+    if (mbar_try_wait(bar, parity) || mbar_wait(bar, parity)) return true;
+    stop = 1;
+    flag(a.b.status, kErrTimeout);
+    return false;
+  };
+  auto tile_col = [&](int t) { return tmem + t * S::TC; };
+
+  if (warp >= S::SOFT && warp < S::SOFT + 4) {
+    // ---- loads
+    registers_down<S::LOAD_REGS>();
+    const int lt = tid - 32 * S::SOFT, lw = warp - S::SOFT;  // 0..127, 0..3
+    const int32_t* row = a.b.table;
+    const KT* kpool = static_cast<const KT*>(a.b.k);
+    const KT* vpool = static_cast<const KT*>(a.b.v);
+    constexpr int EL = 16 / (int)sizeof(KT);             // elements of a 16-byte load
+    constexpr int PER = HD / EL;                         // loads of a key
+    constexpr int NL = KEYS * PER / 128;                 // loads of a thread for a unit's keys
+    const int slot_mask = (1 << a.b.shift) - 1;
+    int i = 0;
+    bool ok = true;
+    for (; ok && w.more(); w.next()) {
+      if (!a.prefix) row = a.b.table + w.p.s * a.b.table_stride;
+      const int all_see = w.seen(w.p.j * S::ROWS / a.b.rep);  // keys that the block's first row sees
+      for (int u = w.p.u0; ok && u < w.p.u1; ++u, ++i) {
+        const int st = i % STG, k0 = u * KEYS;
+        const uint32_t par = ((i / STG) & 1) ^ 1;
+        uint8_t* kd = smem + (size_t)st * 2 * S::HALF;
+        uint8_t* vd = kd + S::HALF;
+        // a unit that every row sees whole, of good pages?
+        const bool whole = k0 + KEYS <= all_see;
+        bool plain = kHalf && whole;
+        if (kHalf) {
+          bool good = true;
+          for (int k = lane << a.b.shift; k < KEYS; k += 32 << a.b.shift)
+            if (k0 + k < w.p.keys) good &= (unsigned)__ldg(row + ((k0 + k) >> a.b.shift)) < (unsigned)a.b.n_pages;
+          plain = __all_sync(0xffffffffu, good) && plain;
+        }
+        ok = load_warps_agree(wait(k_empty + st, par) && wait(v_empty + st, par));
+        if (!ok) break;
+        if (plain) {
+          if (lane == 0 && lw > 0) {
+            mbar_arrive(k_full + st);
+            mbar_arrive(v_full + st);
+          }
+          if (lw == 0) {
+            const int rows = min(KEYS, 1 << a.b.shift), boxes = KEYS / rows;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              uint64_t* bar = h ? v_full + st : k_full + st;
+              if (lane == 0) mbar_expect_tx(bar, S::PART);
+              __syncwarp();
+              for (int x = lane; x < boxes * S::PANELS; x += 32) {
+                const int bx = x / S::PANELS, pn = x - bx * S::PANELS, key = k0 + bx * rows;
+                const int id = __ldg(row + (key >> a.b.shift)), slot = key & slot_mask;
+                const uint32_t dst = smem_u32(h ? vd : kd) + pn * S::PANEL + bx * rows * RB;
+                asm volatile(
+                    "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+                    "%5, %6}], [%7];" ::"r"(dst),
+                    "l"(h ? &maps.v : &maps.k), "r"(0), "r"(pn), "r"(a.swap ? slot : w.p.kv),
+                    "r"(a.swap ? w.p.kv : slot), "r"(id), "r"(smem_u32(bar))
+                    : "memory");
+              }
+            }
+          }
+          continue;
+        }
+        // through registers
+        if (!whole) {
+          if (lt < 4) odd_keys[lt] = 0u;
+          load_warps_agree(true);
+        }
+        constexpr int BATCH = NL < 4 ? NL : 4;
+#pragma unroll 1
+        for (int n0 = 0; n0 < NL; n0 += BATCH) {
+          uint4 rv[BATCH], rk[BATCH];
+#pragma unroll
+          for (int n = 0; n < BATCH; ++n) {
+            const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL;
+            rk[n] = rv[n] = make_uint4(0u, 0u, 0u, 0u);
+            if (k0 + k < w.p.keys) {
+              const int id = __ldg(row + ((k0 + k) >> a.b.shift));
+              if ((unsigned)id < (unsigned)a.b.n_pages) {
+                const int64_t at = id * a.b.page_stride + (int64_t)((k0 + k) & slot_mask) * a.b.slot_stride +
+                                   w.p.kv * a.b.head_stride + e;
+                rv[n] = __ldg(reinterpret_cast<const uint4*>(vpool + at));
+                rk[n] = __ldg(reinterpret_cast<const uint4*>(kpool + at));
+              } else {
+                rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
+                flag(a.b.status, kErrInput);
+              }
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+              const uint32_t* x = reinterpret_cast<const uint32_t*>(&rv[n]);
+              bool odd = false;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                odd |= kHalf ? (x[q] & 0x7C00u) == 0x7C00u || (x[q] & 0x7C000000u) == 0x7C000000u
+                             : (x[q] & 0x7F800000u) == 0x7F800000u;
+              if (odd) {
+                const int k = ((n0 + n) * 128 + lt) / PER;
+                atomicOr(&odd_keys[k >> 5], 1u << (k & 31));
+              }
+            }
+            load_warps_agree(true);
+          }
+#pragma unroll
+          for (int n = 0; n < BATCH; ++n) {
+            const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL;
+            if (!whole && (odd_keys[k >> 5] >> (k & 31) & 1)) {
+              rv[n] = make_uint4(0u, 0u, 0u, 0u);
+              rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
+            }
+            const int col = e * 2, pn = col / RB, at = panel_place<RB>(k, col - pn * RB) + pn * S::PANEL;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint8_t* dst = (h ? kd : vd) + at;
+              const uint4 r = h ? rk[n] : rv[n];
+              if constexpr (kHalf) {
+                *reinterpret_cast<uint4*>(dst) = r;
+              } else {
+                uint32_t lo[3], hi[3];
+                split_pair<false, 3>(__uint_as_float(r.x), __uint_as_float(r.y), lo);
+                split_pair<false, 3>(__uint_as_float(r.z), __uint_as_float(r.w), hi);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(dst + q * S::PART) = make_uint2(lo[q], hi[q]);
+              }
+            }
+          }
+        }
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(k_full + st);
+          mbar_arrive(v_full + st);
+        }
+      }
+    }
+    if (kHalf && lw == 0 && stop) {
+      // copies that are still on their way land before the CTA ends
+      for (int st = 0; st < STG && st < i; ++st) {
+        mbar_wait(k_full + st, ((i - 1 - st) / STG) & 1);
+        mbar_wait(v_full + st, ((i - 1 - st) / STG) & 1);
+      }
+    }
+  } else if (warp >= S::SOFT + 4) {
+    // ---- MMAs
+    registers_down<S::MMA_REGS>();
+    if (warp == S::SOFT + 4 && lane == 0) {
+      constexpr uint32_t kFmt = kHalf ? 0u : 1u;
+      const uint32_t idesc_s = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KEYS >> 3) << 17) | (8u << 24);
+      constexpr int NV = HD < 64 ? HD : 64;  // a V panel's columns
+      const uint32_t idesc_o = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(NV >> 3) << 17) | (8u << 24);
+      const uint32_t base = smem_u32(smem);
+      // products (A part, B part), small ones first
+      constexpr int NPROD = kHalf ? 2 : 6;
+      // (two bits each; rolled loops: unrolled descriptors spill)
+      constexpr uint32_t pa = kHalf ? 0x1u : 0x046u, pb = kHalf ? 0x0u : 0x124u;
+      int i = 0, sn = 0;                 // units; S buffers written
+      uint32_t qn[2] = {0, 0}, pn[2] = {0, 0}, dn[2] = {0, 0};  // waits done on q_full, p_full, pv_done
+      bool ok = true;
+      auto qk = [&](int t, int buf, int st) {
+        const uint32_t d = tile_col(t) + S::QC + (BUFS == 2 ? buf * S::SC : 0) + S::S0;
+#pragma unroll 1
+        for (int x = 0; x < NPROD; ++x) {
+          const uint32_t b0 = base + st * 2 * S::HALF + (pb >> (2 * x) & 3) * S::PART;
+          const uint32_t a0 = tile_col(t) + (pa >> (2 * x) & 3) * (HD / 2);
+#pragma unroll 2
+          for (int k = 0; k < HD / 16; ++k) {
+            const int panel = k * 32 / RB, at = k * 32 - panel * RB;
+            tc::umma_ts(d, a0 + 8 * k, tile_desc<RB>(b0 + panel * S::PANEL + at), idesc_s, (x | k) != 0);
+          }
+        }
+      };
+      auto pv = [&](int t, int buf, int st, bool add) {
+        const uint32_t o = tile_col(t) + S::QC + BUFS * S::SC;
+        const uint32_t p = tile_col(t) + S::QC + (BUFS == 2 ? buf * S::SC : 0);
+#pragma unroll 1
+        for (int x = 0; x < NPROD; ++x) {
+          const uint32_t b0 = base + st * 2 * S::HALF + S::HALF + (pb >> (2 * x) & 3) * S::PART;
+          const uint32_t a0 = p + (pa >> (2 * x) & 3) * 16;
+#pragma unroll 2
+          for (int k = 0; k < KEYS / 16; ++k) {
+            // P: chunks of 32 keys, the parts of a chunk side by side (16 columns each)
+            const uint32_t at = a0 + (k >> 1) * 16 * QP + (k & 1) * 8;
+#pragma unroll
+            for (int h = 0; h < S::PANELS; ++h)
+              tc::umma_ts(o + h * 64, at, tile_desc<RB>(b0 + h * S::PANEL + k * 16 * RB), idesc_o, add || (x | k) != 0);
+          }
+        }
+      };
+      for (; ok && w.more(); w.next()) {
+        const int nt = TILES == 2 && w.rows() > 128 ? 2 : 1;
+        for (int t = 0; ok && t < nt; ++t) ok = wait(q_full + t, qn[t]++ & 1);
+        ok = ok && wait(k_full + i % STG, (i / STG) & 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        // (every earlier PV has been waited for by the softmax, which then gave the new Q)
+        for (int t = 0; t < nt; ++t) {
+          qk(t, sn & 1, i % STG);
+          tc::umma_commit(s_full + (TILES == 2 ? t : sn & 1));
+        }
+        tc::umma_commit(k_empty + i % STG);
+        for (int u = w.p.u0; ok && u < w.p.u1; ++u, ++i) {
+          const int st = i % STG, nst = (i + 1) % STG;
+          const bool add = (u - w.p.u0) % S::kFlush != 0, last = u + 1 == w.p.u1;
+          if (TILES == 1) {
+            // the next unit's S goes to the other buffer, whose P the last PV has read
+            if (!last) {
+              ok = wait(k_full + nst, ((i + 1) / STG) & 1);
+              if (ok && u > w.p.u0) ok = wait(pv_done, dn[0]++ & 1);
+              if (!ok) break;
+              tc::tc_fence_after();
+              qk(0, (sn + 1) & 1, nst);
+              tc::umma_commit(s_full + ((sn + 1) & 1));
+              tc::umma_commit(k_empty + nst);
+            }
+            ok = wait(v_full + st, (i / STG) & 1) && wait(p_full + (sn & 1), pn[sn & 1]++ & 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+            pv(0, sn & 1, st, add);
+            tc::umma_commit(pv_done);
+            tc::umma_commit(v_empty + st);
+            ++sn;
+          } else {
+            ok = wait(v_full + st, (i / STG) & 1);
+            if (ok && !last) ok = wait(k_full + nst, ((i + 1) / STG) & 1);
+            for (int t = 0; ok && t < nt; ++t) {
+              ok = wait(p_full + t, pn[t]++ & 1);
+              if (!ok) break;
+              tc::tc_fence_after();
+              pv(t, 0, st, add);
+              tc::umma_commit(pv_done + t);
+              if (t + 1 == nt) tc::umma_commit(v_empty + st);
+              if (!last) {  // S overlays the P that this PV reads
+                ok = wait(pv_done + t, dn[t]++ & 1);
+                if (!ok) break;
+                tc::tc_fence_after();
+                qk(t, 0, nst);
+                tc::umma_commit(s_full + t);
+                if (t + 1 == nt) tc::umma_commit(k_empty + nst);
+              }
+            }
+          }
+        }
+        // the PVs that this thread has not waited for are the softmax's to wait for
+        if (TILES == 1)
+          dn[0] += w.p.u1 - w.p.u0 > 1 ? 2 : 1;
+        else
+          for (int t = 0; t < nt; ++t) ++dn[t];
+      }
+      tc::umma_commit(&drain);
+      if (!mbar_wait(&drain, 0)) flag(a.b.status, kErrTimeout);
+    }
+  } else {
+    // ---- softmax: one row a thread
+    registers_up<S::SOFT_REGS>();
+    const int t = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t qcol = tile_col(t) + lanes, scol = qcol + S::QC, ocol = scol + BUFS * S::SC;
+    constexpr float kOff = kHalf ? 4.f : 0.f;  // FP16 weights reach 2^(kOff + 8): their low parts stay normal
+    constexpr int NCH = KEYS / 32;
+    uint32_t sn = 0, s_seen[2] = {0, 0}, done = 0;
+    bool ok = true;
+    for (; ok && w.more(); w.next()) {
+      if (TILES == 2 && t == 1 && w.rows() <= 128) continue;
+      const int ri = w.p.j * S::ROWS + t * 128 + r;  // row of the (sequence, kv head)
+      const bool in = t * 128 + r < w.rows();
+      const int tok = ri / a.b.rep, h = w.p.kv * a.b.rep + (ri - tok * a.b.rep);
+      const int64_t token = w.p.tok0 + tok;
+      const int vis = in ? w.seen(tok) : 0;
+      float sc = a.scale;
+      {
+        // Q's parts into tensor memory, two elements a column
+        const float* qp = a.q + token * a.ldq + (int64_t)h * HD;
+        float down = 1.f;
+        if (kHalf) {
+          float mx = 0.f;
+          if (in)
+            for (int e = 0; e < HD; e += 4) {
+              const float4 v = __ldg(reinterpret_cast<const float4*>(qp + e));
+              mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            }
+          const int ex = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
+          down = __uint_as_float((uint32_t)(254 - ex) << 23);
+          sc *= __uint_as_float((uint32_t)ex << 23);
+        }
+#pragma unroll 1
+        for (int e0 = 0; e0 < HD; e0 += 16) {
+          uint32_t part[QP][8];
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in) v = __ldg(reinterpret_cast<const float4*>(qp + e0 + e));
+            uint32_t x[QP], y[QP];
+            split_pair<kHalf, QP>(v.x * down, v.y * down, x);
+            split_pair<kHalf, QP>(v.z * down, v.w * down, y);
+#pragma unroll
+            for (int q = 0; q < QP; ++q) {
+              part[q][e / 2] = x[q];
+              part[q][e / 2 + 1] = y[q];
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < QP; ++q)
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(qcol + q * (HD / 2) + e0 / 2),
+                "r"(part[q][0]), "r"(part[q][1]), "r"(part[q][2]), "r"(part[q][3]), "r"(part[q][4]), "r"(part[q][5]),
+                "r"(part[q][6]), "r"(part[q][7])
+                : "memory");
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full + t);
+      }
+      float acc[HD];
+#pragma unroll
+      for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+      float ref = 0.f, lim = -INFINITY, l = 0.f;
+      for (int u = w.p.u0; ok && u < w.p.u1; ++u) {
+        const int buf = TILES == 2 ? t : (int)(sn & 1);
+        ok = wait(s_full + buf, s_seen[buf]++ & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t pcol = scol + (BUFS == 2 ? (sn & 1) * S::SC : 0);
+        ++sn;
+        const int left = vis - u * KEYS;  // keys of the unit that the row sees
+        const bool masked = !__all_sync(0xffffffffu, left >= KEYS);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < NCH; ++ch) {
+          float v[32];
+          tmem_load(pcol + S::S0 + 32 * ch, v);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * ch + e >= left) v[e] = -INFINITY;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx = fmaxf(mx, v[e]);
+        }
+        mx *= sc;
+        const int uu = u - w.p.u0;
+        const bool flush = uu > 0 && uu % S::kFlush == 0;
+        const bool grow = __any_sync(0xffffffffu, mx - ref > lim);
+        // Every PV is waited for, in order and before the weights that let the next
+        // one start are handed over: a parity tells a phase from its neighbours only.
+        // Here when O is needed, else behind the arithmetic.
+        auto before = [&]() {
+          ok = wait(pv_done + (TILES == 2 ? t : 0), done++ & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          tc::tc_fence_after();
+        };
+        if (uu > 0 && (flush || grow)) {
+          before();
+          if (!ok) break;
+        }
+        if (flush) {
+#pragma unroll
+          for (int d = 0; d < HD; d += 16) {
+            float v[16];
+            tmem_load(ocol + d, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d + e] += v[e];
+          }
+        }
+        if (grow) {
+          const bool seen = lim != -INFINITY;
+          const float m = seen ? fmaxf(mx - kOff, ref) : (mx == -INFINITY ? 0.f : mx - kOff);
+          const float f = seen ? ex2(ref - m) : 1.f;
+          if (mx != -INFINITY) lim = kOff + 8.f;
+          ref = m;
+          l *= f;
+          if (uu > 0 && !flush) {
+#pragma unroll
+            for (int d = 0; d < HD; d += 16) {
+              float v[16];
+              uint32_t x[16];
+              tmem_load(ocol + d, v);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(v[e] * f);
+              tc::tmem_st16(ocol + d, x);
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < HD; ++d) acc[d] *= f;
+        }
+        float l2 = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < NCH; ++ch) {
+          float v[32];
+          tmem_load(pcol + S::S0 + 32 * ch, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(v[e], sc, -ref));
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * ch + e >= left) v[e] = 0.f;
+          }
+          uint32_t part[QP][16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            uint32_t x[QP];
+            l += v[2 * e];
+            l2 += v[2 * e + 1];
+            split_pair<kHalf, QP>(v[2 * e], v[2 * e + 1], x);
+#pragma unroll
+            for (int q = 0; q < QP; ++q) part[q][e] = x[q];
+          }
+#pragma unroll
+          for (int q = 0; q < QP; ++q) tc::tmem_st16(pcol + ch * 16 * QP + q * 16, part[q]);
+        }
+        l += l2;
+        if (uu > 0 && !(flush || grow)) {
+          before();
+          if (!ok) break;
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + buf);
+      }
+      if (ok) {
+        ok = wait(pv_done + (TILES == 2 ? t : 0), done++ & 1);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (!ok) {
+        l = NAN;  // a wait ran out: the rows become NaN
+      } else {
+        tc::tc_fence_after();
+#pragma unroll
+        for (int d = 0; d < HD; d += 16) {
+          float v[16];
+          tmem_load(ocol + d, v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[d + e] += v[e];
+        }
+        tc::tc_fence_before();
+      }
+      if (in) {
+        const bool begin = w.p.u0 == 0, whole = begin && w.p.u1 == w.p.units;
+        const float m = lim == -INFINITY ? -INFINITY : ref;
+        float* dst;
+        float* ml;
+        float inv = 1.f;
+        if (a.prefix) {
+          // piece k of item (kv, j): the CTA's number among the item's
+          const int64_t first = w.p.x - w.p.u0;
+          const int k = (int)(c - owner_of(first, units, workers));
+          const int64_t at = (((int64_t)k * a.items + (int64_t)w.p.kv * w.blocks() + w.p.j) * S::ROWS + t * 128 + r);
+          dst = a.part + at * HD;
+          ml = a.part_ml + at * 2;
+        } else if (!whole) {
+          const int64_t at = (c * 2 + (w.p.x == x0 && !begin ? 0 : 1)) * S::ROWS + t * 128 + r;
+          dst = a.part + at * HD;
+          ml = a.part_ml + at * 2;
+        } else {
+          dst = a.out + (token * a.H + h) * HD;
+          ml = a.state ? a.state + (token * a.H + h) * 2 : nullptr;
+          if (!ml) inv = l == 0.f ? 0.f : 1.f / l;
+        }
+#pragma unroll
+        for (int d = 0; d < HD; d += 4)
+          *reinterpret_cast<float4*>(dst + d) =
+              make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+        if (ml) {
+          ml[0] = m;
+          ml[1] = l;
+        }
+        if (!a.prefix && r == 0 && t == 0 && begin && !whole) {
+          const int64_t lastu = w.p.x - w.p.u0 + w.p.units - 1;
+          a.desc[c * 2] = make_int4(w.p.tok0, w.p.kv, w.p.j, (int)(owner_of(lastu, units, workers) - c) + 1);
+          a.desc[c * 2 + 1] = make_int4(w.rows(), 0, 0, 0);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == S::SOFT + 4) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of blocks that several CTAs hold: block (c, y) takes 16 rows
+// of the item that starts in CTA c, a warp a row at a time.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(128) rows_merge_kernel(TcArgs a) {
+  const int c = blockIdx.x;
+  const int4 d = a.desc[2 * c];
+  if (d.w == 0) return;
+  const int rows = a.desc[2 * c + 1].x, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < 16; i += 4) {
+    const int r = blockIdx.y * 16 + i;
+    if (r >= rows) return;
+    auto at = [&](int k) { return (int64_t)((c + k) * 2 + (k == 0 ? 1 : 0)) * ROWS + r; };
+    float M = -INFINITY;
+    for (int k = lane; k < d.w; k += 32) M = fmaxf(M, a.part_ml[at(k) * 2]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = ref_of(M);
+    float l = 0.f, acc[(HD + 31) / 32] = {};
+    for (int k = 0; k < d.w; ++k) {
+      const float w = ex2(a.part_ml[at(k) * 2] - ref);
+      l += w * a.part_ml[at(k) * 2 + 1];
+#pragma unroll
+      for (int x = 0; x < (HD + 31) / 32; ++x)
+        if (x * 32 + lane < HD) acc[x] = fmaf(w, a.part[at(k) * HD + x * 32 + lane], acc[x]);
+    }
+    const int ri = d.z * ROWS + r, tok = ri / a.b.rep, h = d.y * a.b.rep + ri - tok * a.b.rep;
+    const int64_t row = (int64_t)(d.x + tok) * a.H + h;
+    const float inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+#pragma unroll
+    for (int x = 0; x < (HD + 31) / 32; ++x)
+      if (x * 32 + lane < HD) a.out[row * HD + x * 32 + lane] = acc[x] * inv;
+    if (a.state && lane == 0) {
+      a.state[row * 2] = M;
+      a.state[row * 2 + 1] = l;
+    }
+  }
+}
+
+// Zeros the rows of tokens that no sequence holds.
+__global__ void zero_rows_kernel(Batch b, float* out, int row) {
+  const int lo = b.n > 0 ? min(max(__ldg(b.starts), 0), b.T) : b.T;
+  const int hi = b.n > 0 ? min(max(__ldg(b.starts + b.n), lo), b.T) : b.T;
+  const int64_t per = row / 4, total = (int64_t)(lo + b.T - hi) * per;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / per, tok = t < lo ? t : hi + (t - lo);
+    reinterpret_cast<float4*>(out)[tok * per + (i - t * per)] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
+// Joins a token's own state (output unnormalised, (m, l) in `state`) with the
+// prefix's pieces: one warp a (token, head) row.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(256) prefix_join_kernel(TcArgs a, int64_t units, int workers, int per) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.b.T * a.H) return;
+  const int tok = (int)(row / a.H), h = (int)(row - (int64_t)tok * a.H), kv = h / a.b.rep;
+  if (a.own_rows) {  // ragged: padding rows are not the batch's
+    const int lo = a.b.n > 0 ? __ldg(a.own_rows) : 0, hi = a.b.n > 0 ? __ldg(a.own_rows + a.b.n) : 0;
+    if (tok < lo || tok >= hi) return;
+  }
+  const int ri = tok * a.b.rep + h - kv * a.b.rep, j = ri / ROWS;
+  const int64_t item = (int64_t)kv * (a.items / a.b.kv_heads) + j;
+  const int64_t c0 = owner_of(item * per, units, workers);
+  const int pieces = (int)(owner_of(item * per + per - 1, units, workers) - c0) + 1;
+  auto at = [&](int k) { return ((int64_t)k * a.items + item) * ROWS + (ri - j * ROWS); };
+  const float m0 = a.state[row * 2];
+  float M = m0;
+  for (int k = lane; k < pieces; k += 32) M = fmaxf(M, a.part_ml[at(k) * 2]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = ref_of(M);
+  float w = ex2(m0 - ref), l = w * a.state[row * 2 + 1], acc[(HD + 31) / 32];
+#pragma unroll
+  for (int x = 0; x < (HD + 31) / 32; ++x) acc[x] = x * 32 + lane < HD ? w * a.out[row * HD + x * 32 + lane] : 0.f;
+#pragma unroll 4
+  for (int k = 0; k < pieces; ++k) {
+    w = ex2(a.part_ml[at(k) * 2] - ref);
+    l += w * a.part_ml[at(k) * 2 + 1];
+#pragma unroll
+    for (int x = 0; x < (HD + 31) / 32; ++x)
+      if (x * 32 + lane < HD) acc[x] = fmaf(w, a.part[at(k) * HD + x * 32 + lane], acc[x]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 0; x < (HD + 31) / 32; ++x)
+    if (x * 32 + lane < HD) a.out[row * HD + x * 32 + lane] = acc[x] * inv;
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+template <int HD, typename KT>
+struct TcLaunch {
+  using S = TcShape<HD, KT>;
+
+  static int32_t rows(TcArgs a, cudaStream_t st) {
+    auto kern = rows_kernel<HD, KT>;
+    static std::mutex mu;
+    static bool granted[64] = {false};  // per device
+    int dev = 0;
+    Q6W_CUDA_TRY(cudaGetDevice(&dev));
+    {
+      std::lock_guard<std::mutex> lock(mu);
+      if (!granted[dev & 63]) {
+        // the register split needs all that it divides
+        cudaFuncAttributes attr;
+        Q6W_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
+        if (attr.numRegs != S::REGS)
+          return fail(Q6W_ERR_CUDA, "rows_kernel was built for %d registers a thread, not %d", attr.numRegs, S::REGS);
+        Q6W_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+        granted[dev & 63] = true;
+      }
+    }
+    TcMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    if (S::kHalf) {
+      const int box = std::min(S::KEYS, 1 << a.b.shift);
+      bool swap = false;
+      int32_t rc = pool_map(a.b, a.b.k, HD, 2, 1, box, 1, &maps.k, &swap);
+      if (!rc) rc = pool_map(a.b, a.b.v, HD, 2, 1, box, 1, &maps.v, &swap);
+      if (rc) return rc;
+      a.swap = swap;
+    }
+    kern<<<sm_count(), S::THREADS, S::SMEM, st>>>(a, maps);
+    Q6W_LAUNCH_CHECK("rows_kernel");
+    return Q6W_OK;
+  }
+
+  static int32_t own(TcArgs a, cudaStream_t st) {
+    a.prefix = 0;
+    line_kernel<S::ROWS, S::KEYS><<<1, 1024, 0, st>>>(a, a.line);
+    Q6W_LAUNCH_CHECK("line_kernel");
+    int32_t rc = rows(a, st);
+    if (rc) return rc;
+    rows_merge_kernel<HD, S::ROWS><<<dim3(sm_count(), S::ROWS / 16), 128, 0, st>>>(a);
+    Q6W_LAUNCH_CHECK("rows_merge_kernel");
+    return Q6W_OK;
+  }
+
+  static int per(const TcArgs& a) { return std::max(1, (a.prefix_len + S::KEYS - 1) / S::KEYS); }
+  static int64_t items(const Batch& b) { return (int64_t)b.kv_heads * (((int64_t)b.T * b.rep + S::ROWS - 1) / S::ROWS); }
+  // pieces of an item at most: CTAs that its units can reach
+  static int64_t pieces(const Batch& b, int prefix_len) {
+    const int64_t p = std::max(1, (prefix_len + S::KEYS - 1) / S::KEYS), units = items(b) * p;
+    const int64_t g = std::min<int64_t>(sm_count(), units);
+    return std::min<int64_t>(p, (p * g + units - 1) / units + 1);
+  }
+  static int32_t prefix(TcArgs a, cudaStream_t st) {
+    a.prefix = 1;
+    a.items = (int)items(a.b);
+    return rows(a, st);
+  }
+  static int32_t join(TcArgs a, cudaStream_t st) {
+    a.items = (int)items(a.b);
+    const int64_t units = (int64_t)a.items * per(a);
+    const int64_t total = (int64_t)a.b.T * a.H;
+    prefix_join_kernel<HD, S::ROWS><<<(unsigned)((total + 7) / 8), 256, 0, st>>>(
+        a, units, (int)std::min<int64_t>(sm_count(), units), per(a));
+    Q6W_LAUNCH_CHECK("prefix_join_kernel");
+    return Q6W_OK;
+  }
+  static size_t own_rows() { return (size_t)sm_count() * 2 * S::ROWS; }
+  static size_t prefix_rows(const Batch& b, int prefix_len) { return (size_t)(pieces(b, prefix_len) * items(b)) * S::ROWS; }
+};
+
+#define Q6W_TC_DISPATCH(hd, half, call)                                             \
+  switch (hd) {                                                                     \
+    case 16: return half ? TcLaunch<16, __half>::call : TcLaunch<16, float>::call;  \
+    case 32: return half ? TcLaunch<32, __half>::call : TcLaunch<32, float>::call;  \
+    case 64: return half ? TcLaunch<64, __half>::call : TcLaunch<64, float>::call;  \
+    default: return half ? TcLaunch<128, __half>::call : TcLaunch<128, float>::call; \
+  }
+
+int32_t rows_own(const TcArgs& a, int hd, bool half, cudaStream_t st) { Q6W_TC_DISPATCH(hd, half, own(a, st)) }
+int32_t rows_prefix(const TcArgs& a, int hd, bool half, cudaStream_t st) { Q6W_TC_DISPATCH(hd, half, prefix(a, st)) }
+int32_t rows_join(const TcArgs& a, int hd, bool half, cudaStream_t st) { Q6W_TC_DISPATCH(hd, half, join(a, st)) }
+size_t rows_own_rows(int hd, bool half) { Q6W_TC_DISPATCH(hd, half, own_rows()) }
+size_t rows_prefix_rows(const Batch& b, int prefix_len, int hd, bool half) {
+  Q6W_TC_DISPATCH(hd, half, prefix_rows(b, prefix_len))
+}
+
+int32_t zero_padding_rows(const Batch& b, float* out, int row, cudaStream_t st) {
+  const int64_t vecs = (int64_t)b.T * row / 4;
+  zero_rows_kernel<<<(unsigned)std::min<int64_t>((vecs + 255) / 256, (int64_t)sm_count() * 4), 256, 0, st>>>(b, out, row);
+  Q6W_LAUNCH_CHECK("zero_rows_kernel");
+  return Q6W_OK;
+}
+
+}  // namespace paged
+}  // namespace q6w
