@@ -78,9 +78,9 @@ struct TcShape {
   // (what the block was launched with, 64 K / THREADS a thread, divided anew).
   static constexpr int THREADS = 32 * (SOFT + 8);
   static constexpr int REGS = TILES == 2 ? 128 : 168;
-  static constexpr int SOFT_REGS = TILES == 2 ? 168 : 240, LOAD_REGS = TILES == 2 ? 104 : 160, MMA_REGS = TILES == 2 ? 72 : 104;
+  static constexpr int SOFT_REGS = TILES == 2 ? (kHalf ? 168 : 152) : 240, LOAD_REGS = TILES == 2 ? (kHalf ? 104 : 136) : 184, MMA_REGS = TILES == 2 ? 72 : 80;
   static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
-  static constexpr int kFlush = 4;
+  static constexpr int kFlush = kHalf ? 4 : 1;  // units between additions of O to registers
   static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
 };
 
@@ -136,14 +136,13 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) {
                : "memory");
 }
 
-// A thread's registers from here on (a whole group of four warps calls it).
-template <int N>
-__device__ __forceinline__ void registers_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void registers_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+// A thread's registers from here on, `FROM` before (a whole group of four warps calls it).
+template <int FROM, int TO>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (TO > FROM)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
+  else if constexpr (TO < FROM)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
 }
 
 // The AND of `ok` over the four load warps (all of them call it).
@@ -388,7 +387,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
 
   if (warp >= S::SOFT && warp < S::SOFT + 4) {
     // ---- loads
-    registers_down<S::LOAD_REGS>();
+    set_registers<S::REGS, S::LOAD_REGS>();
     const int lt = tid - 32 * S::SOFT, lw = warp - S::SOFT;  // 0..127, 0..3
     const int32_t* row = a.b.table;
     const KT* kpool = static_cast<const KT*>(a.b.k);
@@ -399,6 +398,81 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     const int slot_mask = (1 << a.b.shift) - 1;
     int i = 0;
     bool ok = true;
+    // Units through registers, BATCH loads of keys and values a thread at a time.
+    constexpr int MOST = kHalf ? 4 : 8, BATCH = NL < MOST ? NL : MOST;
+    uint4 rv[BATCH], rk[BATCH];
+    auto fetch = [&](const Piece& p, int u, int n0, int n) {
+      const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL, key = u * KEYS + k;
+      rk[n] = rv[n] = make_uint4(0u, 0u, 0u, 0u);
+      if (key < p.keys) {
+        const int id = __ldg((a.prefix ? a.b.table : a.b.table + p.s * a.b.table_stride) + (key >> a.b.shift));
+        if ((unsigned)id < (unsigned)a.b.n_pages) {
+          const int64_t at = id * a.b.page_stride + (int64_t)(key & slot_mask) * a.b.slot_stride + p.kv * a.b.head_stride + e;
+          rv[n] = __ldg(reinterpret_cast<const uint4*>(vpool + at));
+          rk[n] = __ldg(reinterpret_cast<const uint4*>(kpool + at));
+        } else {
+          rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
+          flag(a.b.status, kErrInput);
+        }
+      }
+    };
+    auto store = [&](uint8_t* kd, uint8_t* vd, bool whole, int n0, int n) {
+      const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL;
+      if (!whole && (odd_keys[k >> 5] >> (k & 31) & 1)) {
+        rv[n] = make_uint4(0u, 0u, 0u, 0u);
+        rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
+      }
+      const int col = e * 2, pn = col / RB, at = panel_place<RB>(k, col - pn * RB) + pn * S::PANEL;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint8_t* dst = (h ? kd : vd) + at;
+        const uint4 r = h ? rk[n] : rv[n];
+        if constexpr (kHalf) {
+          *reinterpret_cast<uint4*>(dst) = r;
+        } else {
+          uint32_t lo[3], hi[3];
+          split_pair<false, 3>(__uint_as_float(r.x), __uint_as_float(r.y), lo);
+          split_pair<false, 3>(__uint_as_float(r.z), __uint_as_float(r.w), hi);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(dst + q * S::PART) = make_uint2(lo[q], hi[q]);
+        }
+      }
+    };
+    // keys of the batch whose values are not finite
+    auto mark = [&](int n0) {
+#pragma unroll
+      for (int n = 0; n < BATCH; ++n) {
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(&rv[n]);
+        bool odd = false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          odd |= kHalf ? (x[q] & 0x7C00u) == 0x7C00u || (x[q] & 0x7C000000u) == 0x7C000000u
+                       : (x[q] & 0x7F800000u) == 0x7F800000u;
+        if (odd) {
+          const int k = ((n0 + n) * 128 + lt) / PER;
+          atomicOr(&odd_keys[k >> 5], 1u << (k & 31));
+        }
+      }
+      load_warps_agree(true);
+    };
+    // FP32 units all go this way: a batch's registers are loaded again, with the
+    // batch behind it (the next unit's, over the ends of pieces), as they are stored.
+    Walk<S::ROWS, KEYS> ahead(a);
+    ahead.p = w.p;
+    ahead.end = w.end;
+    int au = w.p.u0, an = 0;
+    auto ahead_next = [&]() {
+      if ((an += BATCH) < NL) return;
+      an = 0;
+      if (++au < ahead.p.u1) return;
+      ahead.next();
+      au = ahead.p.u0;
+    };
+    if (!kHalf && ahead.more()) {
+#pragma unroll
+      for (int n = 0; n < BATCH; ++n) fetch(ahead.p, au, an, n);
+      ahead_next();
+    }
     for (; ok && w.more(); w.next()) {
       if (!a.prefix) row = a.b.table + w.p.s * a.b.table_stride;
       const int all_see = w.seen(w.p.j * S::ROWS / a.b.rep);  // keys that the block's first row sees
@@ -450,66 +524,19 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           if (lt < 4) odd_keys[lt] = 0u;
           load_warps_agree(true);
         }
-        constexpr int BATCH = NL < 4 ? NL : 4;
 #pragma unroll 1
         for (int n0 = 0; n0 < NL; n0 += BATCH) {
-          uint4 rv[BATCH], rk[BATCH];
+          if (kHalf) {
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) fetch(w.p, u, n0, n);
+          }
+          if (!whole) mark(n0);
 #pragma unroll
           for (int n = 0; n < BATCH; ++n) {
-            const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL;
-            rk[n] = rv[n] = make_uint4(0u, 0u, 0u, 0u);
-            if (k0 + k < w.p.keys) {
-              const int id = __ldg(row + ((k0 + k) >> a.b.shift));
-              if ((unsigned)id < (unsigned)a.b.n_pages) {
-                const int64_t at = id * a.b.page_stride + (int64_t)((k0 + k) & slot_mask) * a.b.slot_stride +
-                                   w.p.kv * a.b.head_stride + e;
-                rv[n] = __ldg(reinterpret_cast<const uint4*>(vpool + at));
-                rk[n] = __ldg(reinterpret_cast<const uint4*>(kpool + at));
-              } else {
-                rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
-                flag(a.b.status, kErrInput);
-              }
-            }
+            store(kd, vd, whole, n0, n);
+            if (!kHalf && ahead.more()) fetch(ahead.p, au, an, n);
           }
-          if (!whole) {
-#pragma unroll
-            for (int n = 0; n < BATCH; ++n) {
-              const uint32_t* x = reinterpret_cast<const uint32_t*>(&rv[n]);
-              bool odd = false;
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                odd |= kHalf ? (x[q] & 0x7C00u) == 0x7C00u || (x[q] & 0x7C000000u) == 0x7C000000u
-                             : (x[q] & 0x7F800000u) == 0x7F800000u;
-              if (odd) {
-                const int k = ((n0 + n) * 128 + lt) / PER;
-                atomicOr(&odd_keys[k >> 5], 1u << (k & 31));
-              }
-            }
-            load_warps_agree(true);
-          }
-#pragma unroll
-          for (int n = 0; n < BATCH; ++n) {
-            const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL;
-            if (!whole && (odd_keys[k >> 5] >> (k & 31) & 1)) {
-              rv[n] = make_uint4(0u, 0u, 0u, 0u);
-              rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
-            }
-            const int col = e * 2, pn = col / RB, at = panel_place<RB>(k, col - pn * RB) + pn * S::PANEL;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint8_t* dst = (h ? kd : vd) + at;
-              const uint4 r = h ? rk[n] : rv[n];
-              if constexpr (kHalf) {
-                *reinterpret_cast<uint4*>(dst) = r;
-              } else {
-                uint32_t lo[3], hi[3];
-                split_pair<false, 3>(__uint_as_float(r.x), __uint_as_float(r.y), lo);
-                split_pair<false, 3>(__uint_as_float(r.z), __uint_as_float(r.w), hi);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(dst + q * S::PART) = make_uint2(lo[q], hi[q]);
-              }
-            }
-          }
+          if (!kHalf && ahead.more()) ahead_next();
         }
         tc::fence_async_smem();
         __syncwarp();
@@ -528,7 +555,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     }
   } else if (warp >= S::SOFT + 4) {
     // ---- MMAs
-    registers_down<S::MMA_REGS>();
+    set_registers<S::REGS, S::MMA_REGS>();
     if (warp == S::SOFT + 4 && lane == 0) {
       constexpr uint32_t kFmt = kHalf ? 0u : 1u;
       const uint32_t idesc_s = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KEYS >> 3) << 17) | (8u << 24);
@@ -637,7 +664,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     }
   } else {
     // ---- softmax: one row a thread
-    registers_up<S::SOFT_REGS>();
+    set_registers<S::REGS, S::SOFT_REGS>();
     const int t = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t qcol = tile_col(t) + lanes, scol = qcol + S::QC, ocol = scol + BUFS * S::SC;

@@ -7,7 +7,8 @@ raises ``Q6WLibraryError``.
 
 import ctypes
 import os
-from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_void_p
+import struct
+from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_NAME = "libq6w_b200.so"
@@ -75,13 +76,8 @@ class GreedyArgs(ctypes.Structure):
                 ("step_logits", c_void_p), ("prefill_event", c_void_p)]
 
 
-class PagedBatch(ctypes.Structure):
-    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("kv_dtype", c_int32), ("n_pages", c_int32),
-                ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_stride", c_int64),
-                ("slot_stride", c_int64), ("head_stride", c_int64), ("n_seqs", c_int32), ("max_pages", c_int32),
-                ("page_table", c_void_p), ("table_stride", c_int64), ("lengths", c_void_p),
-                ("query_starts", c_void_p), ("status", c_void_p)]
-
+# q6w_paged_batch, in native alignment (packing it costs a third of filling a ctypes.Structure)
+PAGED_BATCH = struct.Struct("@PPiiiiiqqqiiPqPPP")
 
 _lib = None
 _load_error = None
@@ -122,12 +118,12 @@ def _declare(lib):
                                       c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, S]),
         "q6w_prefill": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int64, c_void_p,
                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t, S]),
-        "q6w_paged_append": (c_int32, [POINTER(PagedBatch), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64,
+        "q6w_paged_append": (c_int32, [c_char_p, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64,
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, S]),
-        "q6w_paged_workspace_bytes": (c_size_t, [POINTER(PagedBatch), c_int32, c_int32, c_int32]),
-        "q6w_paged_attention": (c_int32, [POINTER(PagedBatch), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int32,
+        "q6w_paged_workspace_bytes": (c_size_t, [c_char_p, c_int32, c_int32, c_int32]),
+        "q6w_paged_attention": (c_int32, [c_char_p, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int32,
                                           c_void_p, c_size_t, S]),
-        "q6w_shared_prefix_attention": (c_int32, [POINTER(PagedBatch), c_void_p, c_int32, c_int32, c_int32, c_void_p,
+        "q6w_shared_prefix_attention": (c_int32, [c_char_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
                                                   c_int64, c_void_p, c_int32, c_void_p, c_size_t, S]),
         "q6w_gqa_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int64, S]),

@@ -272,66 +272,80 @@ def gqa_attention(queries, keys, values, lengths, groups_per_kv):
 
 # ---- serving from a paged cache -------------------------------------------------
 
-_KV_DTYPES = {torch.float32: 0, torch.float16: 1}
+_I32, _F32, _F16 = torch.int32, torch.float32, torch.float16
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (a build without CUDA has none)
 
 
-def _int32(name, t, device, dim):
-    if t.dtype != torch.int32 or t.device != device or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be an int32 tensor of {dim} dimension(s) on {device} with contiguous rows")
+def _int32(name, t, dev, dim):
+    """Address of an int32 tensor with contiguous rows on device ``dev``."""
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name} must be an int32 tensor of {dim} dimension(s) on cuda:{dev} with contiguous rows")
     return t.data_ptr()
 
 
-def _token_rows(name, t, heads, hd, device):
-    """Token stride of t [T, heads, hd] FP32: heads contiguous, tokens at any stride."""
-    if t.dtype != torch.float32 or t.device != device or t.dim() != 3 or t.shape[2] != hd or (
-            heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be float32 [tokens, heads, {hd}] on {device}")
-    T, H, _ = t.shape
-    st = t.stride()
-    if t.numel() and (st[2] != 1 or (H > 1 and st[1] != hd)):
+def _token_rows(name, t, heads, hd, dev):
+    """(tokens, heads, token stride) of t [T, heads, hd] FP32: heads contiguous, tokens at any stride."""
+    if t.dtype is not _F32 or t.get_device() != dev or t.dim() != 3:
+        raise ValueError(f"{name} must be float32 [tokens, heads, {hd}] on cuda:{dev}")
+    T, H, d = t.shape
+    st, sh, sd = t.stride()
+    if d != hd or (heads is not None and H != heads):
+        raise ValueError(f"{name} must be float32 [tokens, heads, {hd}] on cuda:{dev}")
+    if T and (sd != 1 or (sh != hd and H > 1)):
         raise ValueError(f"the heads of a token of {name} must be contiguous")
-    return st[0] if T > 1 else H * hd
+    return T, H, st if T > 1 else H * hd
 
 
 def _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, n_tokens):
-    device = key_pages.device
-    if device.type != "cuda":
+    """(q6w_paged_batch as bytes, device index, kv_heads, head_dim)."""
+    dev = key_pages.get_device()
+    if dev < 0:
         raise ValueError("q6w_b200 ops run on CUDA devices only")
-    kv = _KV_DTYPES.get(key_pages.dtype)
-    if kv is None or value_pages.dtype != key_pages.dtype or value_pages.device != device:
+    dtype = key_pages.dtype
+    if (dtype is not _F32 and dtype is not _F16) or value_pages.dtype is not dtype or value_pages.get_device() != dev:
         raise ValueError("key_pages and value_pages must both be float32 or float16 on one device")
-    if key_pages.dim() != 4 or value_pages.shape != key_pages.shape or value_pages.stride() != key_pages.stride():
+    strides = key_pages.stride()
+    if len(strides) != 4 or value_pages.shape != key_pages.shape or value_pages.stride() != strides:
         raise ValueError("key_pages and value_pages must be [pages, page_size, kv_heads, head_dim] with equal strides")
     pages, page_size, kv_heads, hd = key_pages.shape
-    sp, ss, sh, sd = key_pages.stride()
+    sp, ss, sh, sd = strides
     if sd != 1:
         raise ValueError("the last dimension of the pages must be contiguous")
-    table = _int32("page_table", page_table, device, 2)
+    table = _int32("page_table", page_table, dev, 2)
     n, width = page_table.shape
-    lens = _int32("lengths", lengths, device, 1)
+    lens = _int32("lengths", lengths, dev, 1)
     if lengths.shape[0] != n:
         raise ValueError(f"lengths must have one entry for each of the {n} rows of page_table")
-    starts = None
+    starts = flags = 0
     if query_starts is not None:
-        starts = _int32("query_starts", query_starts, device, 1)
+        starts = _int32("query_starts", query_starts, dev, 1)
         if query_starts.shape[0] != n + 1:
             raise ValueError(f"query_starts must have {n + 1} entries")
     elif n_tokens != n:
         raise ValueError(f"{n_tokens} tokens of {n} sequences need query_starts")
-    flags = None if status is None else _int32("status", status, device, 1)
-    if status is not None and status.shape[0] < 1:
-        raise ValueError("status must have an entry")
-    return _lib.PagedBatch(key_pages.data_ptr(), value_pages.data_ptr(), kv, pages, page_size, kv_heads, hd, sp, ss, sh,
-                           n, width, table, page_table.stride(0), lens, starts, flags)
+    if status is not None:
+        flags = _int32("status", status, dev, 1)
+        if status.shape[0] < 1:
+            raise ValueError("status must have an entry")
+    return _lib.PAGED_BATCH.pack(key_pages.data_ptr(), value_pages.data_ptr(), 0 if dtype is _F32 else 1, pages, page_size,
+                                 kv_heads, hd, sp, ss, sh, n, width, table, page_table.stride(0), lens, starts,
+                                 flags), dev, kv_heads, hd
 
 
-def _on_device(device):
-    """Make ``device`` current for a call; nothing to do when it is."""
-    import contextlib
+def _on_device(dev, call, *args):
+    """``call(*args, stream)`` with device ``dev`` and its current stream."""
+    if torch._C._cuda_getDevice() == dev:
+        return call(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return call(*args, _raw_stream(dev))
 
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+
+def _rows_out(out, queries, T, H, hd, dev):
+    if out is None:
+        return queries.new_empty((T, H, hd))
+    if out.shape != queries.shape or out.dtype is not _F32 or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous float32 of the queries' shape")
+    return out
 
 
 def paged_append(queries, keys, values, cos, sin, key_pages, value_pages, page_table, lengths, query_starts=None,
@@ -355,35 +369,29 @@ def paged_append(queries, keys, values, cos, sin, key_pages, value_pages, page_t
     ``status``: int32 [1] on the device, zeroed once; bit 0 is set when a
     length, page id or position is out of range (``check_status``).
     """
-    device = key_pages.device
     T = keys.shape[0]
-    b = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
-    kv_heads, hd = b.kv_heads, b.head_dim
-    ldk = _token_rows("keys", keys, kv_heads, hd, device)
-    ldv = _token_rows("values", values, kv_heads, hd, device)
-    if values.shape[0] != T or (queries is not None and queries.shape[0] != T):
-        raise ValueError("queries, keys and values must have the same number of tokens")
-    for t in (cos, sin):
-        if t.dtype != torch.float32 or t.device != device or t.dim() != 2 or t.shape[1] * 2 != hd or not t.is_contiguous():
-            raise ValueError(f"cos and sin must be contiguous float32 [positions, {hd // 2}] on {device}")
-    if cos.shape != sin.shape:
-        raise ValueError("cos and sin must have the same shape")
+    batch, dev, kv_heads, hd = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
+    ldk = _token_rows("keys", keys, kv_heads, hd, dev)[2]
+    Tv, _, ldv = _token_rows("values", values, kv_heads, hd, dev)
     H = ldq = 0
     q = rot = None
+    Tq = T
     zero = out is None
     if queries is not None:
-        ldq = _token_rows("queries", queries, None, hd, device)
-        H = queries.shape[1]
-        if zero:
-            out = torch.empty((T, H, hd), dtype=torch.float32, device=device)
-        elif out.shape != queries.shape or out.dtype != torch.float32 or out.device != device or not out.is_contiguous():
-            raise ValueError("out must be contiguous float32 of the queries' shape")
+        Tq, H, ldq = _token_rows("queries", queries, None, hd, dev)
+        out = _rows_out(out, queries, Tq, H, hd, dev)
         q, rot = queries.data_ptr(), out.data_ptr()
+    if Tv != T or Tq != T:
+        raise ValueError("queries, keys and values must have the same number of tokens")
+    positions = cos.shape
+    if (cos.dtype is not _F32 or sin.dtype is not _F32 or cos.get_device() != dev or sin.get_device() != dev
+            or len(positions) != 2 or positions[1] * 2 != hd or sin.shape != positions or not cos.is_contiguous()
+            or not sin.is_contiguous()):
+        raise ValueError(f"cos and sin must be contiguous float32 [positions, {hd // 2}] on cuda:{dev}")
     lib = _lib.load()
-    with _on_device(device):
-        _lib.check(lib.q6w_paged_append(b, T, H, q, ldq, keys.data_ptr(), ldk, values.data_ptr(), ldv, cos.data_ptr(),
-                                        sin.data_ptr(), cos.shape[0], int(first_position), rot, zero,
-                                        _lib.stream_handle()), "q6w_paged_append")
+    _lib.check(_on_device(dev, lib.q6w_paged_append, batch, T, H, q, ldq, keys.data_ptr(), ldk, values.data_ptr(), ldv,
+                          cos.data_ptr(), sin.data_ptr(), positions[0], int(first_position), rot, zero),
+               "q6w_paged_append")
     return out if queries is not None else None
 
 
@@ -410,7 +418,7 @@ def shared_prefix_attention(queries, key_pages, value_pages, prefix_pages, prefi
     own tokens (a length may be 0); their positions start at prefix_length
     (``paged_append(..., first_position=prefix_length)``).
     """
-    pages = _int32("prefix_pages", prefix_pages, key_pages.device, 1)
+    pages = _int32("prefix_pages", prefix_pages, key_pages.get_device(), 1)
     if prefix_length < 0 or prefix_length > prefix_pages.shape[0] * key_pages.shape[1]:
         raise ValueError("prefix_length is more than prefix_pages hold")
     return _paged_attention(queries, key_pages, value_pages, pages, int(prefix_length), page_table, lengths,
@@ -419,28 +427,18 @@ def shared_prefix_attention(queries, key_pages, value_pages, prefix_pages, prefi
 
 def _paged_attention(queries, key_pages, value_pages, prefix_pages, prefix_length, page_table, lengths, query_starts,
                      status, out):
-    device = key_pages.device
-    T, H = queries.shape[:2]
-    b = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
-    hd = b.head_dim
-    ldq = _token_rows("queries", queries, None, hd, device)
+    batch, dev, _, hd = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, queries.shape[0])
+    T, H, ldq = _token_rows("queries", queries, None, hd, dev)
     zero = out is None
-    if zero:
-        out = torch.empty((T, H, hd), dtype=torch.float32, device=device)
-    elif out.shape != queries.shape or out.dtype != torch.float32 or out.device != device or not out.is_contiguous():
-        raise ValueError("out must be contiguous float32 of the queries' shape")
+    out = _rows_out(out, queries, T, H, hd, dev)
     lib = _lib.load()
-    with _on_device(device):
-        need = lib.q6w_paged_workspace_bytes(b, T, H, prefix_length)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _lib.check(lib.q6w_shared_prefix_attention(b, prefix_pages, prefix_length, T, H, queries.data_ptr(), ldq,
-                                                   out.data_ptr(), zero, ws.data_ptr() if need else None, need,
-                                                   _lib.stream_handle()), "paged attention")
+    need = lib.q6w_paged_workspace_bytes(batch, T, H, prefix_length)
+    ws = key_pages.new_empty(need, dtype=torch.uint8)  # (stream-ordered: a call's own, released as it returns)
+    _lib.check(_on_device(dev, lib.q6w_shared_prefix_attention, batch, prefix_pages, prefix_length, T, H,
+                          queries.data_ptr(), ldq, out.data_ptr(), zero, ws.data_ptr(), need), "paged attention")
     return out
 
 
 def check_status(status):
     """Synchronise and raise Q6WError if a paged call set ``status`` (then clear it)."""
-    lib = _lib.load()
-    with _on_device(status.device):
-        _lib.check(lib.q6w_workspace_status(status.data_ptr(), _lib.stream_handle()), "paged cache")
+    _lib.check(_on_device(status.get_device(), _lib.load().q6w_workspace_status, status.data_ptr()), "paged cache")
