@@ -61,6 +61,9 @@ struct TcShape {
   static constexpr int KEYS = kHalf ? 128 : 64;
   static constexpr int QP = kHalf ? 2 : 3;         // parts of Q and P
   static constexpr int KP = kHalf ? 1 : 3;         // parts of K and V
+  // product x takes part pa(x) of A and pb(x) of B
+  static constexpr int pa(int x) { return kHalf ? 1 - x : (0x046 >> 2 * x) & 3; }
+  static constexpr int pb(int x) { return kHalf ? 0 : (0x124 >> 2 * x) & 3; }
   static constexpr int RB = HD * 2 < 128 ? HD * 2 : 128;  // bytes of a panel row = swizzle span
   static constexpr int PANELS = HD * 2 / RB;
   static constexpr int PANEL = KEYS * RB;
@@ -88,11 +91,41 @@ struct TcShape {
 // groups `group` bytes apart.  (K-major: the groups are along the keys, the MMA's
 // N; MN-major: along the keys too, its K; both offsets are given the same
 // stride, as the other one is not used by operands one swizzle span wide.)
+// Its upper word is a constant, its lower word grows by bytes / 16 with the address.
 template <int RB>
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
-  constexpr uint64_t layout = RB == 128 ? 2 : RB == 64 ? 4 : 6;
-  constexpr uint64_t group = RB * 8 / 16;
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (group << 16) | (group << 32) | (1ull << 46) | (layout << 61);
+struct TileDesc {
+  static constexpr uint32_t group = RB * 8 / 16;
+  static constexpr uint32_t hi = group | (1u << 14) | ((RB == 128 ? 2u : RB == 64 ? 4u : 6u) << 29);
+  __device__ static __forceinline__ uint32_t lo(uint32_t addr) { return (addr >> 4) | (group << 16); }
+};
+
+// D (tensor memory) += A (tensor memory, a + ADD) B (shared memory, b + BDD);
+// `add` false: D = A B.  The constants are added inside, not held in registers.
+template <int ADD, int BDD, uint32_t HI>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 bd;\n\t.reg .b32 al, bl;\n\t"
+      "add.u32 al, %1, %5;\n\tadd.u32 bl, %2, %6;\n\t"
+      "mov.b64 bd, {bl, %7};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [al], bd, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(ADD), "n"(BDD), "n"(HI)
+      : "memory");
+}
+// True in one lane of the (converged) warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// f(0), f(1), .. f(N - 1) with the index a constant.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(const F& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    unrolled<N, I + 1>(f);
+  }
 }
 
 // Byte place of byte `at` of row `row` in a swizzled panel.
@@ -395,21 +428,28 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     constexpr int EL = 16 / (int)sizeof(KT);             // elements of a 16-byte load
     constexpr int PER = HD / EL;                         // loads of a key
     constexpr int NL = KEYS * PER / 128;                 // loads of a thread for a unit's keys
-    const int slot_mask = (1 << a.b.shift) - 1;
+    const int slot_mask = (1 << a.b.shift) - 1, slot_stride = (int)a.b.slot_stride, head_stride = (int)a.b.head_stride;
     int i = 0;
     bool ok = true;
     // Units through registers, BATCH loads of keys and values a thread at a time.
     constexpr int MOST = kHalf ? 4 : 8, BATCH = NL < MOST ? NL : MOST;
     uint4 rv[BATCH], rk[BATCH];
+    int ids[BATCH];  // page ids of the batch to fetch
+    auto pages = [&](const Piece& p, int u, int n0) {
+#pragma unroll
+      for (int n = 0; n < BATCH; ++n) {
+        const int key = u * KEYS + ((n0 + n) * 128 + lt) / PER;
+        ids[n] = key < p.keys ? __ldg((a.prefix ? a.b.table : a.b.table + p.s * a.b.table_stride) + (key >> a.b.shift)) : -1;
+      }
+    };
     auto fetch = [&](const Piece& p, int u, int n0, int n) {
       const int idx = (n0 + n) * 128 + lt, k = idx / PER, e = (idx - k * PER) * EL, key = u * KEYS + k;
       rk[n] = rv[n] = make_uint4(0u, 0u, 0u, 0u);
       if (key < p.keys) {
-        const int id = __ldg((a.prefix ? a.b.table : a.b.table + p.s * a.b.table_stride) + (key >> a.b.shift));
-        if ((unsigned)id < (unsigned)a.b.n_pages) {
-          const int64_t at = id * a.b.page_stride + (int64_t)(key & slot_mask) * a.b.slot_stride + p.kv * a.b.head_stride + e;
-          rv[n] = __ldg(reinterpret_cast<const uint4*>(vpool + at));
-          rk[n] = __ldg(reinterpret_cast<const uint4*>(kpool + at));
+        if ((unsigned)ids[n] < (unsigned)a.b.n_pages) {
+          const int64_t at = ids[n] * a.b.page_stride + ((key & slot_mask) * slot_stride + p.kv * head_stride + e);
+          rv[n] = __ldcg(reinterpret_cast<const uint4*>(vpool + at));
+          rk[n] = __ldcg(reinterpret_cast<const uint4*>(kpool + at));
         } else {
           rk[n] = make_uint4(~0u, ~0u, ~0u, ~0u);
           flag(a.b.status, kErrInput);
@@ -469,9 +509,11 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       au = ahead.p.u0;
     };
     if (!kHalf && ahead.more()) {
+      pages(ahead.p, au, an);
 #pragma unroll
       for (int n = 0; n < BATCH; ++n) fetch(ahead.p, au, an, n);
       ahead_next();
+      if (ahead.more()) pages(ahead.p, au, an);
     }
     for (; ok && w.more(); w.next()) {
       if (!a.prefix) row = a.b.table + w.p.s * a.b.table_stride;
@@ -527,6 +569,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
 #pragma unroll 1
         for (int n0 = 0; n0 < NL; n0 += BATCH) {
           if (kHalf) {
+            pages(w.p, u, n0);
 #pragma unroll
             for (int n = 0; n < BATCH; ++n) fetch(w.p, u, n0, n);
           }
@@ -536,7 +579,10 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
             store(kd, vd, whole, n0, n);
             if (!kHalf && ahead.more()) fetch(ahead.p, au, an, n);
           }
-          if (!kHalf && ahead.more()) ahead_next();
+          if (!kHalf && ahead.more()) {
+            ahead_next();
+            if (ahead.more()) pages(ahead.p, au, an);
+          }
         }
         tc::fence_async_smem();
         __syncwarp();
@@ -556,7 +602,10 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   } else if (warp >= S::SOFT + 4) {
     // ---- MMAs
     set_registers<S::REGS, S::MMA_REGS>();
-    if (warp == S::SOFT + 4 && lane == 0) {
+    if (warp == S::SOFT + 4) {
+      // The whole warp walks and waits, one elected lane issues: inside its branch
+      // the MMA's operands stay in uniform registers (issued by a lone lane of a
+      // diverged warp, every MMA took 100 cycles whatever its size).
       constexpr uint32_t kFmt = kHalf ? 0u : 1u;
       const uint32_t idesc_s = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KEYS >> 3) << 17) | (8u << 24);
       constexpr int NV = HD < 64 ? HD : 64;  // a V panel's columns
@@ -564,102 +613,112 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       const uint32_t base = smem_u32(smem);
       // products (A part, B part), small ones first
       constexpr int NPROD = kHalf ? 2 : 6;
-      // (two bits each; rolled loops: unrolled descriptors spill)
-      constexpr uint32_t pa = kHalf ? 0x1u : 0x046u, pb = kHalf ? 0x0u : 0x124u;
+      using Desc = TileDesc<RB>;
       int i = 0, sn = 0;                 // units; S buffers written
       uint32_t qn[2] = {0, 0}, pn[2] = {0, 0}, dn[2] = {0, 0};  // waits done on q_full, p_full, pv_done
       bool ok = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait(bar, parity)); };
       auto qk = [&](int t, int buf, int st) {
         const uint32_t d = tile_col(t) + S::QC + (BUFS == 2 ? buf * S::SC : 0) + S::S0;
-#pragma unroll 1
-        for (int x = 0; x < NPROD; ++x) {
-          const uint32_t b0 = base + st * 2 * S::HALF + (pb >> (2 * x) & 3) * S::PART;
-          const uint32_t a0 = tile_col(t) + (pa >> (2 * x) & 3) * (HD / 2);
-#pragma unroll 2
-          for (int k = 0; k < HD / 16; ++k) {
-            const int panel = k * 32 / RB, at = k * 32 - panel * RB;
-            tc::umma_ts(d, a0 + 8 * k, tile_desc<RB>(b0 + panel * S::PANEL + at), idesc_s, (x | k) != 0);
-          }
-        }
+        const uint32_t lo = Desc::lo(base + st * 2 * S::HALF), q = tile_col(t);
+        unrolled<NPROD * (HD / 16)>([&](auto ic) {
+          constexpr int x = ic.value / (HD / 16), k = ic.value % (HD / 16);
+          constexpr int panel = k * 32 / RB, at = k * 32 - panel * RB;
+          mma_ts<S::pa(x) * (HD / 2) + 8 * k, (S::pb(x) * S::PART + panel * S::PANEL + at) / 16, Desc::hi>(d, q, lo, idesc_s,
+                                                                                                  (x | k) != 0);
+        });
       };
       auto pv = [&](int t, int buf, int st, bool add) {
         const uint32_t o = tile_col(t) + S::QC + BUFS * S::SC;
         const uint32_t p = tile_col(t) + S::QC + (BUFS == 2 ? buf * S::SC : 0);
-#pragma unroll 1
-        for (int x = 0; x < NPROD; ++x) {
-          const uint32_t b0 = base + st * 2 * S::HALF + S::HALF + (pb >> (2 * x) & 3) * S::PART;
-          const uint32_t a0 = p + (pa >> (2 * x) & 3) * 16;
-#pragma unroll 2
-          for (int k = 0; k < KEYS / 16; ++k) {
-            // P: chunks of 32 keys, the parts of a chunk side by side (16 columns each)
-            const uint32_t at = a0 + (k >> 1) * 16 * QP + (k & 1) * 8;
-#pragma unroll
-            for (int h = 0; h < S::PANELS; ++h)
-              tc::umma_ts(o + h * 64, at, tile_desc<RB>(b0 + h * S::PANEL + k * 16 * RB), idesc_o, add || (x | k) != 0);
-          }
-        }
+        const uint32_t lo = Desc::lo(base + st * 2 * S::HALF + S::HALF);
+        unrolled<NPROD * (KEYS / 16)>([&](auto ic) {
+          constexpr int x = ic.value / (KEYS / 16), k = ic.value % (KEYS / 16);
+          // P: chunks of 32 keys, the parts of a chunk side by side (16 columns each)
+          unrolled<S::PANELS>([&](auto hc) {
+            constexpr int h = hc.value;
+            mma_ts<(k >> 1) * 16 * QP + S::pa(x) * 16 + (k & 1) * 8, (S::pb(x) * S::PART + h * S::PANEL + k * 16 * RB) / 16,
+                   Desc::hi>(o + h * 64, p, lo, idesc_o, add || (x | k) != 0);
+          });
+        });
       };
       for (; ok && w.more(); w.next()) {
         const int nt = TILES == 2 && w.rows() > 128 ? 2 : 1;
-        for (int t = 0; ok && t < nt; ++t) ok = wait(q_full + t, qn[t]++ & 1);
-        ok = ok && wait(k_full + i % STG, (i / STG) & 1);
+        for (int t = 0; ok && t < nt; ++t) ok = wait_all(q_full + t, qn[t]++ & 1);
+        ok = ok && wait_all(k_full + i % STG, (i / STG) & 1);
         if (!ok) break;
         tc::tc_fence_after();
         // (every earlier PV has been waited for by the softmax, which then gave the new Q)
-        for (int t = 0; t < nt; ++t) {
-          qk(t, sn & 1, i % STG);
-          tc::umma_commit(s_full + (TILES == 2 ? t : sn & 1));
+        if (elect_one()) {
+          for (int t = 0; t < nt; ++t) {
+            qk(t, sn & 1, i % STG);
+            tc::umma_commit(s_full + (TILES == 2 ? t : sn & 1));
+          }
+          tc::umma_commit(k_empty + i % STG);
         }
-        tc::umma_commit(k_empty + i % STG);
+        __syncwarp();
         for (int u = w.p.u0; ok && u < w.p.u1; ++u, ++i) {
           const int st = i % STG, nst = (i + 1) % STG;
           const bool add = (u - w.p.u0) % S::kFlush != 0, last = u + 1 == w.p.u1;
           if (TILES == 1) {
             // the next unit's S goes to the other buffer, whose P the last PV has read
             if (!last) {
-              ok = wait(k_full + nst, ((i + 1) / STG) & 1);
-              if (ok && u > w.p.u0) ok = wait(pv_done, dn[0]++ & 1);
+              ok = wait_all(k_full + nst, ((i + 1) / STG) & 1);
+              if (ok && u > w.p.u0) ok = wait_all(pv_done, dn[0]++ & 1);
               if (!ok) break;
               tc::tc_fence_after();
-              qk(0, (sn + 1) & 1, nst);
-              tc::umma_commit(s_full + ((sn + 1) & 1));
-              tc::umma_commit(k_empty + nst);
+              if (elect_one()) {
+                qk(0, (sn + 1) & 1, nst);
+                tc::umma_commit(s_full + ((sn + 1) & 1));
+                tc::umma_commit(k_empty + nst);
+              }
+              __syncwarp();
             }
-            ok = wait(v_full + st, (i / STG) & 1) && wait(p_full + (sn & 1), pn[sn & 1]++ & 1);
+            ok = wait_all(v_full + st, (i / STG) & 1) && wait_all(p_full + (sn & 1), pn[sn & 1]++ & 1);
             if (!ok) break;
             tc::tc_fence_after();
-            pv(0, sn & 1, st, add);
-            tc::umma_commit(pv_done);
-            tc::umma_commit(v_empty + st);
+            if (elect_one()) {
+              pv(0, sn & 1, st, add);
+              tc::umma_commit(pv_done);
+              tc::umma_commit(v_empty + st);
+            }
+            __syncwarp();
             ++sn;
           } else {
-            ok = wait(v_full + st, (i / STG) & 1);
-            if (ok && !last) ok = wait(k_full + nst, ((i + 1) / STG) & 1);
+            ok = wait_all(v_full + st, (i / STG) & 1);
+            if (ok && !last) ok = wait_all(k_full + nst, ((i + 1) / STG) & 1);
             for (int t = 0; ok && t < nt; ++t) {
-              ok = wait(p_full + t, pn[t]++ & 1);
+              ok = wait_all(p_full + t, pn[t]++ & 1);
               if (!ok) break;
               tc::tc_fence_after();
-              pv(t, 0, st, add);
-              tc::umma_commit(pv_done + t);
-              if (t + 1 == nt) tc::umma_commit(v_empty + st);
+              if (elect_one()) {
+                pv(t, 0, st, add);
+                tc::umma_commit(pv_done + t);
+                if (t + 1 == nt) tc::umma_commit(v_empty + st);
+              }
+              __syncwarp();
               if (!last) {  // S overlays the P that this PV reads
-                ok = wait(pv_done + t, dn[t]++ & 1);
+                ok = wait_all(pv_done + t, dn[t]++ & 1);
                 if (!ok) break;
                 tc::tc_fence_after();
-                qk(t, 0, nst);
-                tc::umma_commit(s_full + t);
-                if (t + 1 == nt) tc::umma_commit(k_empty + nst);
+                if (elect_one()) {
+                  qk(t, 0, nst);
+                  tc::umma_commit(s_full + t);
+                  if (t + 1 == nt) tc::umma_commit(k_empty + nst);
+                }
+                __syncwarp();
               }
             }
           }
         }
-        // the PVs that this thread has not waited for are the softmax's to wait for
+        // the PVs that this warp has not waited for are the softmax's to wait for
         if (TILES == 1)
           dn[0] += w.p.u1 - w.p.u0 > 1 ? 2 : 1;
         else
           for (int t = 0; t < nt; ++t) ++dn[t];
       }
-      tc::umma_commit(&drain);
+      if (elect_one()) tc::umma_commit(&drain);
+      __syncwarp();
       if (!mbar_wait(&drain, 0)) flag(a.b.status, kErrTimeout);
     }
   } else {
