@@ -26,7 +26,8 @@
 // tiles in a CTA (head_dim <= 64) the softmax of one runs under the MMAs of the
 // other, with one tile (head_dim 128) S has two buffers.
 //
-// Roles: warps 0-3 (4-7) softmax of a tile, then four load warps, one MMA warp.
+// Roles: eight softmax warps (four a tile; with one tile two threads a row, each
+// half of the keys and of O), four load warps, one MMA warp.
 // Load warps fetch FP16 units by TMA boxes; FP32 units, units with a bad page
 // id and units that some row does not see whole go through registers: keys no
 // row sees become zeros, and a key whose value is not finite becomes a NaN key
@@ -76,27 +77,30 @@ struct TcShape {
   static constexpr int S0 = kHalf ? 0 : 32;        // S inside its buffer (P's first chunk stays in front of unread S)
   static constexpr int TC = QC + BUFS * SC + (HD < 32 ? 32 : HD);
   static_assert(TC * TILES <= 512, "tensor memory columns");
-  static constexpr int SOFT = 4 * TILES;           // softmax warps
+  static constexpr int HALVES = 3 - TILES;         // threads of a row: each takes half of the keys and of O
+  static constexpr int SOFT = 8;                   // softmax warps
   // Softmax, load and MMA warps in groups of four with registers of their own
   // (what the block was launched with, 64 K / THREADS a thread, divided anew).
   static constexpr int THREADS = 32 * (SOFT + 8);
-  static constexpr int REGS = TILES == 2 ? 128 : 168;
-  static constexpr int SOFT_REGS = TILES == 2 ? (kHalf ? 168 : 152) : 240, LOAD_REGS = TILES == 2 ? (kHalf ? 104 : 136) : 184, MMA_REGS = TILES == 2 ? 72 : 80;
+  static constexpr int REGS = 128;
+  static constexpr int SOFT_REGS = kHalf ? 168 : 152, LOAD_REGS = kHalf ? 104 : 136, MMA_REGS = 72;
   static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
   static constexpr int kFlush = kHalf ? 4 : 1;  // units between additions of O to registers
   static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
 };
 
 // One MMA shared-memory descriptor: rows of RB bytes swizzled over RB, eight-row
-// groups `group` bytes apart.  (K-major: the groups are along the keys, the MMA's
-// N; MN-major: along the keys too, its K; both offsets are given the same
-// stride, as the other one is not used by operands one swizzle span wide.)
-// Its upper word is a constant, its lower word grows by bytes / 16 with the address.
+// groups RB * 8 bytes apart -- along the MMA's N for the K-major operand (which
+// uses no other offset), along its K for the MN-major one, whose panels (spans of
+// N) stand `panel` bytes apart.  The upper word is a constant, the lower word
+// grows by bytes / 16 with the address.
 template <int RB>
 struct TileDesc {
   static constexpr uint32_t group = RB * 8 / 16;
   static constexpr uint32_t hi = group | (1u << 14) | ((RB == 128 ? 2u : RB == 64 ? 4u : 6u) << 29);
-  __device__ static __forceinline__ uint32_t lo(uint32_t addr) { return (addr >> 4) | (group << 16); }
+  __device__ static __forceinline__ uint32_t lo(uint32_t addr, int panel = 0) {
+    return (addr >> 4) | ((panel ? panel / 16 : group) << 16);
+  }
 };
 
 // D (tensor memory) += A (tensor memory, a + ADD) B (shared memory, b + BDD);
@@ -365,6 +369,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   __shared__ uint64_t q_full[TILES], s_full[2], p_full[2], pv_done[TILES], drain;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int stop;
+  __shared__ float row_max[S::HALVES][2][128], row_sum[S::HALVES][128];  // what a row's two threads tell one another
   __shared__ uint32_t odd_keys[4];  // keys of the unit whose values are not finite
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -381,12 +386,12 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       mbar_init(v_empty + i, 1);
     }
     for (int i = 0; i < TILES; ++i) {
-      mbar_init(q_full + i, 4);
+      mbar_init(q_full + i, 4 * S::HALVES);
       mbar_init(pv_done + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(p_full + i, 4 * S::HALVES);
     }
     mbar_init(&drain, 1);
     stop = 0;
@@ -608,8 +613,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       // diverged warp, every MMA took 100 cycles whatever its size).
       constexpr uint32_t kFmt = kHalf ? 0u : 1u;
       const uint32_t idesc_s = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KEYS >> 3) << 17) | (8u << 24);
-      constexpr int NV = HD < 64 ? HD : 64;  // a V panel's columns
-      const uint32_t idesc_o = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(NV >> 3) << 17) | (8u << 24);
+      const uint32_t idesc_o = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
       const uint32_t base = smem_u32(smem);
       // products (A part, B part), small ones first
       constexpr int NPROD = kHalf ? 2 : 6;
@@ -631,15 +635,12 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       auto pv = [&](int t, int buf, int st, bool add) {
         const uint32_t o = tile_col(t) + S::QC + BUFS * S::SC;
         const uint32_t p = tile_col(t) + S::QC + (BUFS == 2 ? buf * S::SC : 0);
-        const uint32_t lo = Desc::lo(base + st * 2 * S::HALF + S::HALF);
+        const uint32_t lo = Desc::lo(base + st * 2 * S::HALF + S::HALF, S::PANELS > 1 ? S::PANEL : 0);
         unrolled<NPROD * (KEYS / 16)>([&](auto ic) {
           constexpr int x = ic.value / (KEYS / 16), k = ic.value % (KEYS / 16);
           // P: chunks of 32 keys, the parts of a chunk side by side (16 columns each)
-          unrolled<S::PANELS>([&](auto hc) {
-            constexpr int h = hc.value;
-            mma_ts<(k >> 1) * 16 * QP + S::pa(x) * 16 + (k & 1) * 8, (S::pb(x) * S::PART + h * S::PANEL + k * 16 * RB) / 16,
-                   Desc::hi>(o + h * 64, p, lo, idesc_o, add || (x | k) != 0);
-          });
+          mma_ts<(k >> 1) * 16 * QP + S::pa(x) * 16 + (k & 1) * 8, (S::pb(x) * S::PART + k * 16 * RB) / 16, Desc::hi>(
+              o, p, lo, idesc_o, add || (x | k) != 0);
         });
       };
       for (; ok && w.more(); w.next()) {
@@ -724,11 +725,30 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   } else {
     // ---- softmax: one row a thread
     set_registers<S::REGS, S::SOFT_REGS>();
-    const int t = warp >> 2, r = tid & 127;
+    constexpr int HALVES = S::HALVES;
+    const int t = TILES == 2 ? warp >> 2 : 0, hf = HALVES == 2 ? warp >> 2 : 0, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t qcol = tile_col(t) + lanes, scol = qcol + S::QC, ocol = scol + BUFS * S::SC;
+    const uint32_t qcol = tile_col(t) + lanes, scol = qcol + S::QC, ocol = scol + BUFS * S::SC + hf * (HD / HALVES);
     constexpr float kOff = kHalf ? 4.f : 0.f;  // FP16 weights reach 2^(kOff + 8): their low parts stay normal
-    constexpr int NCH = KEYS / 32;
+    constexpr int NCH = KEYS / 32 / HALVES;    // 32-key chunks of a unit that this thread takes
+    constexpr int MYD = HD / HALVES;           // dims of O that this thread takes
+    const int ch0 = hf * NCH;
+    // With two threads a row, a warp and its partner (the same rows' other half)
+    // pass the same barriers: both see the same verdict and stop together.
+    auto agree = [&](bool mine) -> bool {
+      mine = __all_sync(0xffffffffu, mine);
+      if constexpr (HALVES == 2) {
+        uint32_t v;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.aligned.pred q, %2, 64, p;\n\t"
+            "selp.u32 %0, 1, 0, q;\n\t}"
+            : "=r"(v)
+            : "r"((uint32_t)mine), "r"(2 + (warp & 3))
+            : "memory");
+        return v != 0;
+      }
+      return mine;
+    };
     uint32_t sn = 0, s_seen[2] = {0, 0}, done = 0;
     bool ok = true;
     for (; ok && w.more(); w.next()) {
@@ -755,7 +775,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           sc *= __uint_as_float((uint32_t)ex << 23);
         }
 #pragma unroll 1
-        for (int e0 = 0; e0 < HD; e0 += 16) {
+        for (int e0 = hf * MYD; e0 < (hf + 1) * MYD; e0 += 16) {
           uint32_t part[QP][8];
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
@@ -783,33 +803,45 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full + t);
       }
-      float acc[HD];
+      float acc[MYD];
 #pragma unroll
-      for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+      for (int d = 0; d < MYD; ++d) acc[d] = 0.f;
       float ref = 0.f, lim = -INFINITY, l = 0.f;
-      for (int u = w.p.u0; ok && u < w.p.u1; ++u) {
+      for (int u = w.p.u0; u < w.p.u1; ++u) {
         const int buf = TILES == 2 ? t : (int)(sn & 1);
-        ok = wait(s_full + buf, s_seen[buf]++ & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        ok = wait(s_full + buf, s_seen[buf]++ & 1) && ok;
+        if (HALVES == 1) {
+          ok = agree(ok);
+          if (!ok) break;
+        }
         tc::tc_fence_after();
         const uint32_t pcol = scol + (BUFS == 2 ? (sn & 1) * S::SC : 0);
-        ++sn;
         const int left = vis - u * KEYS;  // keys of the unit that the row sees
         const bool masked = !__all_sync(0xffffffffu, left >= KEYS);
+        // Scores are read twice; FP32 rows of two threads keep them, as P overlaps the
+        // scores of the other half.
+        constexpr bool kKeep = HALVES == 2 && !kHalf;
+        float keep[kKeep ? NCH : 1][32];
         float mx = -INFINITY;
 #pragma unroll
         for (int ch = 0; ch < NCH; ++ch) {
-          float v[32];
-          tmem_load(pcol + S::S0 + 32 * ch, v);
+          float(&v)[32] = keep[kKeep ? ch : 0];
+          tmem_load(pcol + S::S0 + 32 * (ch0 + ch), v);
           if (masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (32 * ch + e >= left) v[e] = -INFINITY;
+              if (32 * (ch0 + ch) + e >= left) v[e] = -INFINITY;
           }
 #pragma unroll
           for (int e = 0; e < 32; ++e) mx = fmaxf(mx, v[e]);
         }
+        if constexpr (HALVES == 2) {
+          row_max[hf][sn & 1][r] = mx;
+          ok = agree(ok);
+          if (!ok) break;
+          mx = fmaxf(mx, row_max[hf ^ 1][sn & 1][r]);
+        }
+        ++sn;
         mx *= sc;
         const int uu = u - w.p.u0;
         const bool flush = uu > 0 && uu % S::kFlush == 0;
@@ -818,17 +850,13 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         // one start are handed over: a parity tells a phase from its neighbours only.
         // Here when O is needed, else behind the arithmetic.
         auto before = [&]() {
-          ok = wait(pv_done + (TILES == 2 ? t : 0), done++ & 1);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = __all_sync(0xffffffffu, wait(pv_done + (TILES == 2 ? t : 0), done++ & 1)) && ok;
           tc::tc_fence_after();
         };
-        if (uu > 0 && (flush || grow)) {
-          before();
-          if (!ok) break;
-        }
+        if (uu > 0 && (flush || grow)) before();
         if (flush) {
 #pragma unroll
-          for (int d = 0; d < HD; d += 16) {
+          for (int d = 0; d < MYD; d += 16) {
             float v[16];
             tmem_load(ocol + d, v);
 #pragma unroll
@@ -844,7 +872,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           l *= f;
           if (uu > 0 && !flush) {
 #pragma unroll
-            for (int d = 0; d < HD; d += 16) {
+            for (int d = 0; d < MYD; d += 16) {
               float v[16];
               uint32_t x[16];
               tmem_load(ocol + d, v);
@@ -854,19 +882,19 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
             }
           }
 #pragma unroll
-          for (int d = 0; d < HD; ++d) acc[d] *= f;
+          for (int d = 0; d < MYD; ++d) acc[d] *= f;
         }
         float l2 = 0.f;
 #pragma unroll
         for (int ch = 0; ch < NCH; ++ch) {
-          float v[32];
-          tmem_load(pcol + S::S0 + 32 * ch, v);
+          float(&v)[32] = keep[kKeep ? ch : 0];
+          if (!kKeep) tmem_load(pcol + S::S0 + 32 * (ch0 + ch), v);
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(v[e], sc, -ref));
           if (masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (32 * ch + e >= left) v[e] = 0.f;
+              if (32 * (ch0 + ch) + e >= left) v[e] = 0.f;
           }
           uint32_t part[QP][16];
 #pragma unroll
@@ -879,28 +907,25 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
             for (int q = 0; q < QP; ++q) part[q][e] = x[q];
           }
 #pragma unroll
-          for (int q = 0; q < QP; ++q) tc::tmem_st16(pcol + ch * 16 * QP + q * 16, part[q]);
+          for (int q = 0; q < QP; ++q) tc::tmem_st16(pcol + (ch0 + ch) * 16 * QP + q * 16, part[q]);
         }
         l += l2;
-        if (uu > 0 && !(flush || grow)) {
-          before();
-          if (!ok) break;
-        }
+        if (uu > 0 && !(flush || grow)) before();
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + buf);
       }
-      if (ok) {
-        ok = wait(pv_done + (TILES == 2 ? t : 0), done++ & 1);
-        ok = __all_sync(0xffffffffu, ok);
-      }
+      if (ok) ok = wait(pv_done + (TILES == 2 ? t : 0), done++ & 1);
+      if constexpr (HALVES == 2) row_sum[hf][r] = l;
+      ok = agree(ok);
+      if constexpr (HALVES == 2) l += row_sum[hf ^ 1][r];
       if (!ok) {
         l = NAN;  // a wait ran out: the rows become NaN
       } else {
         tc::tc_fence_after();
 #pragma unroll
-        for (int d = 0; d < HD; d += 16) {
+        for (int d = 0; d < MYD; d += 16) {
           float v[16];
           tmem_load(ocol + d, v);
 #pragma unroll
@@ -931,14 +956,14 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           if (!ml) inv = l == 0.f ? 0.f : 1.f / l;
         }
 #pragma unroll
-        for (int d = 0; d < HD; d += 4)
-          *reinterpret_cast<float4*>(dst + d) =
+        for (int d = 0; d < MYD; d += 4)
+          *reinterpret_cast<float4*>(dst + hf * MYD + d) =
               make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
-        if (ml) {
+        if (ml && hf == 0) {
           ml[0] = m;
           ml[1] = l;
         }
-        if (!a.prefix && r == 0 && t == 0 && begin && !whole) {
+        if (!a.prefix && r == 0 && t == 0 && hf == 0 && begin && !whole) {
           const int64_t lastu = w.p.x - w.p.u0 + w.p.units - 1;
           a.desc[c * 2] = make_int4(w.p.tok0, w.p.kv, w.p.j, (int)(owner_of(lastu, units, workers) - c) + 1);
           a.desc[c * 2 + 1] = make_int4(w.rows(), 0, 0, 0);
