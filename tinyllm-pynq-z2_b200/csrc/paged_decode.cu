@@ -119,6 +119,12 @@ struct DecodeMaps {
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 
+// a b / c, in 32 bits when the product fits (a 64-bit division is a long subroutine).
+__device__ __forceinline__ int64_t muldiv(int64_t a, int64_t b, int64_t c) {
+  const int64_t p = a * b;
+  return (p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)c) : p / c;
+}
+
 // The line of units: prefix sums over 256 stretches of sequences.
 struct Line {
   int64_t pref[kDecodeThreads];
@@ -138,12 +144,18 @@ template <int KU>
 __device__ __forceinline__ void build_line(const Batch& b, Line& line) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (b.n + kDecodeThreads - 1) / kDecodeThreads;
-  int64_t sum = 0;
-  for (int s = tid * seg; s < min((tid + 1) * seg, b.n); ++s) {
+  auto units_at = [&](int s) {
     const int len = __ldg(b.lengths + s);
     if (len > b.max_len) flag(b.status, kErrInput);
-    sum += units_of<KU>(min(max(len, 0), b.max_len));
-  }
+    return units_of<KU>(min(max(len, 0), b.max_len));
+  };
+  int64_t sum = 0;
+  const int first = tid * seg, last = min(first + seg, b.n);
+  int i = first;
+  for (; i + 8 <= last; i += 8)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += units_at(i + k);
+  for (; i < last; ++i) sum += units_at(i);
   int64_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -233,6 +245,10 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // N bytes of shared memory as 32-bit words.
 template <int N>
 __device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&w)[N / 4]) {
@@ -302,13 +318,17 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   const int g = lane >> 2, c = lane & 3;  // the MMA fragments' row group and column group
   const int STATE = state_floats(a.hd);
   uint64_t* bar = bars + warp * STG;
+  if (threadIdx.x == 0) {
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
   if (lane < STG) mbar_init(bar + lane, 1);
   fence_mbar_init();
   build_line<S::KU>(b, line);
   const int KVB = b.kv_heads / a.F * a.HB;
   const int64_t units = line.total * KVB;
   // few units: spread them over the CTAs first, over a CTA's warps second
-  const int aw = (int)min((int64_t)kDecodeWarps, (units + gridDim.x - 1) / gridDim.x);
+  const int aw = units >= (int64_t)gridDim.x * kDecodeWarps ? kDecodeWarps : (int)(((uint32_t)units + gridDim.x - 1) / gridDim.x);
   const int64_t workers = min((int64_t)gridDim.x * aw, units);
   const int64_t wi = (int64_t)blockIdx.x * aw + warp;
   const bool active = warp < aw && wi < workers;
@@ -316,14 +336,14 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   float* slots = a.wpart + ((size_t)blockIdx.x * kDecodeWarps + warp) * 2 * STATE;
   if (active) {
     Cursor<S::KU> cur;
-    cur.x = wi * units / workers;
-    cur.x1 = (wi + 1) * units / workers;
+    cur.x = muldiv(wi, units, workers);
+    cur.x1 = muldiv(wi + 1, units, workers);
     const int64_t xb = cur.x;
-    find_seq<S::KU>(b, line, cur.x / KVB, lane, cur.s, cur.first);
+    find_seq<S::KU>(b, line, muldiv(cur.x, 1, KVB), lane, cur.s, cur.first);
     cur.keys = keys_of(b, cur.s);
     cur.us = units_of<S::KU>(cur.keys);
-    cur.block = (int)((cur.x - cur.first * KVB) / cur.us);
-    cur.u0 = (int)((cur.x - cur.first * KVB) % cur.us);
+    cur.block = (int)muldiv(cur.x - cur.first * KVB, 1, cur.us);
+    cur.u0 = (int)(cur.x - cur.first * KVB - (int64_t)cur.block * cur.us);
     cur.piece();
 
     // ---- loads
@@ -672,6 +692,13 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   if (threadIdx.x == 0) a.desc[blockIdx.x].z = 0;
   const float* pieces = a.wpart + (size_t)blockIdx.x * kDecodeWarps * 2 * STATE;
   const int hd = a.hd, M0 = 8 * hd, L0 = 8 * hd + 8;
+  __shared__ float pm[2 * kDecodeWarps][8], pl[2 * kDecodeWarps][8];
+  if (threadIdx.x < 16 * kDecodeWarps) {
+    const int k = threadIdx.x >> 3, r = threadIdx.x & 7;
+    pm[k][r] = segs[k].valid ? pieces[k * STATE + M0 + r] : -INFINITY;
+    pl[k][r] = segs[k].valid ? pieces[k * STATE + L0 + r] : 0.f;
+  }
+  __syncthreads();
   for (int i = 0; i < 2 * kDecodeWarps;) {
     if (!segs[i].valid) {
       ++i;
@@ -688,27 +715,33 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     int h0, nr;
     block_heads(a, f.block, h0, nr);
     float* dst = a.part + ((size_t)blockIdx.x * 2 + (f.begin ? 1 : 0)) * STATE;
-    for (int x = threadIdx.x; x < nr * hd; x += kDecodeThreads) {
+    for (int x = threadIdx.x * 4; x < nr * hd; x += kDecodeThreads * 4) {
       const int r = x / hd;
       float M = -INFINITY;
-      for (int k = i; k <= last; ++k)
-        if (segs[k].valid) M = fmaxf(M, pieces[k * STATE + M0 + r]);
+      for (int k = i; k <= last; ++k) M = fmaxf(M, pm[k][r]);
       const float ref = ref_of(M);
-      float o = 0.f, l = 0.f;
-      for (int k = i; k <= last; ++k)
-        if (segs[k].valid) {
-          const float* p = pieces + k * STATE;
-          const float w = ex2(p[M0 + r] - ref);
-          o += w * p[x];
-          l += w * p[L0 + r];
-        }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2 * kDecodeWarps; ++n) {
+        if (n < i || n > last || !segs[n].valid) continue;
+        const float w = ex2(pm[n][r] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(pieces + n * STATE + x);
+        o.x = fmaf(w, v.x, o.x);
+        o.y = fmaf(w, v.y, o.y);
+        o.z = fmaf(w, v.z, o.z);
+        o.w = fmaf(w, v.w, o.w);
+        l = fmaf(w, pl[n][r], l);
+      }
+      const bool head = x == r * hd;
       if (f.begin && end) {
         const int64_t row = (int64_t)f.s * a.H + h0;
-        a.out[row * hd + x] = a.state ? o : (l == 0.f ? 0.f : o / l);
-        if (a.state && x % hd == 0) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(M, l);
+        const float inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        *reinterpret_cast<float4*>(a.out + row * hd + x) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (a.state && head) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(M, l);
       } else {
-        dst[x] = o;
-        if (x % hd == 0) {
+        *reinterpret_cast<float4*>(dst + x) = o;
+        if (head) {
           dst[M0 + r] = M;
           dst[L0 + r] = l;
         }
