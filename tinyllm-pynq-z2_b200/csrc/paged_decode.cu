@@ -132,6 +132,11 @@ struct Line {
   int64_t warp_sum[kDecodeWarps];
 };
 
+// Sequences of a stretch.
+__device__ __forceinline__ int stretch(int n) {
+  return n <= kDecodeThreads ? 1 : ((n + kDecodeThreads - 1) / kDecodeThreads + 31) & ~31;
+}
+
 // Keys that sequence s's token sees.
 __device__ __forceinline__ int keys_of(const Batch& b, int s) { return min(max(__ldg(b.lengths + s), 0), b.max_len); }
 
@@ -143,19 +148,37 @@ __device__ __forceinline__ int units_of(int keys) {
 template <int KU>
 __device__ __forceinline__ void build_line(const Batch& b, Line& line) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seg = (b.n + kDecodeThreads - 1) / kDecodeThreads;
-  auto units_at = [&](int s) {
-    const int len = __ldg(b.lengths + s);
-    if (len > b.max_len) flag(b.status, kErrInput);
+  const int seg = stretch(b.n);
+  int64_t sum = 0;
+  bool over = false;
+  auto units_at = [&](int len) {
+    over |= len > b.max_len;
     return units_of<KU>(min(max(len, 0), b.max_len));
   };
-  int64_t sum = 0;
-  const int first = tid * seg, last = min(first + seg, b.n);
-  int i = first;
-  for (; i + 8 <= last; i += 8)
+  if (seg == 1) {
+    if (tid < b.n) sum = units_at(__ldg(b.lengths + tid));
+  } else {
+    // a stretch is a number of 32-sequence rows: a coalesced load and a warp-wide
+    // addition each (a sequence has fewer than 2^27 units), eight loads in flight
+    const int per = seg >> 5;
+    const int64_t first = (int64_t)warp * 32 * seg;
+    for (int g = 0; g < 32 * per && first + g * 32 < b.n; g += 8) {
+      int len[8];
+      bool in[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += units_at(i + k);
-  for (; i < last; ++i) sum += units_at(i);
+      for (int k = 0; k < 8; ++k) {
+        const int64_t s = first + (g + k) * 32 + lane;
+        in[k] = g + k < 32 * per && s < b.n;
+        len[k] = in[k] ? __ldg(b.lengths + s) : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const unsigned u = __reduce_add_sync(0xffffffffu, in[k] ? (unsigned)units_at(len[k]) : 0u);
+        if ((g + k) / per == lane) sum += u;
+      }
+    }
+  }
+  if (over) flag(b.status, kErrInput);
   int64_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -183,7 +206,7 @@ __device__ __forceinline__ void find_seq(const Batch& b, const Line& line, int64
   for (int i = 0; i < kDecodeThreads / 32; ++i) c += line.pref[i * 32 + lane] <= z;
 #pragma unroll
   for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-  const int seg = (b.n + kDecodeThreads - 1) / kDecodeThreads;
+  const int seg = stretch(b.n);
   s = (c - 1) * seg;
   first = line.pref[c - 1];
   for (;;) {
