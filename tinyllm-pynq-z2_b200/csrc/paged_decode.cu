@@ -55,7 +55,7 @@ __host__ __device__ constexpr int state_floats(int hd) { return 8 * hd + 16; }
 
 // First query head and heads of an item's block.
 __device__ __forceinline__ void block_heads(const DecodeArgs& a, int block, int& h0, int& nr) {
-  const int kb = block / a.HB, hb = block - kb * a.HB;
+  const int kb = a.HB == 1 ? block : block / a.HB, hb = block - kb * a.HB;
   h0 = kb * a.F * a.b.rep + hb * a.per;
   nr = a.F > 1 ? a.F * a.b.rep : min(a.per, a.b.rep - hb * a.per);
 }
@@ -340,6 +340,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;  // the MMA fragments' row group and column group
   const int STATE = state_floats(a.hd);
+  // of the F kv heads side by side: head g's, heads 2 c and 2 c + 1's
+  const int fg = a.F > 1 ? g / b.rep : 0, fc[2] = {a.F > 1 ? 2 * c / b.rep : 0, a.F > 1 ? (2 * c + 1) / b.rep : 0};
+  const int hd_shift = 31 - __clz(a.hd);
   uint64_t* bar = bars + warp * STG;
   if (threadIdx.x == 0) {
     prefetch_map(&maps.k);
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       while (p.x < p.x1 && p.key0 >= p.key1) p.next(b, KVB);
       if (p.x >= p.x1) return;
       pt = p.key0;
-      pblk = p.block / a.HB;
+      pblk = a.HB == 1 ? p.block : p.block / a.HB;
       row = b.table + p.s * b.table_stride;
       pbase = p.key0 >> b.shift;
       plast = (p.key1 - 1) >> b.shift;
@@ -462,7 +465,6 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       int h0, nr;
       block_heads(a, cur.block, h0, nr);
       // ---- queries: head g of the block, dims as the lane's key chunks hold them
-      const int fg = a.F > 1 ? g / b.rep : 0;  // its kv head among the F
       uint32_t qhi[2 * QS], qlo[2 * QS];       // step s: words 2 s, 2 s + 1
       float sc0 = a.scale, sc1 = a.scale;      // score scales of heads 2 c, 2 c + 1
       {
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
           const int D = j * 4 * EK + c * EK;
-          const bool in = g < nr && (a.F == 1 || D / a.hd == fg);
+          const bool in = g < nr && (a.F == 1 || D >> hd_shift == fg);
 #pragma unroll
           for (int e = 0; e < EK; e += 4) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
         const int n = 2 * c + hh;
         const float l = hh ? l1 : l0;
         const float inv = !whole || a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-        const int f = a.F > 1 ? n / b.rep : 0;
+        const int f = fc[hh];
         float* dst = whole ? a.out + ((int64_t)s * a.H + h0 + n) * a.hd : slot + n * a.hd;
         if (n < nr) {
 #pragma unroll
@@ -710,6 +712,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       for (int i = 0; i < STG; ++i) mbar_wait(bar + i, phase);
     }
   }
+  grid_dep_launch();
   __syncthreads();
   // ---- pieces of items inside this CTA, in order
   if (threadIdx.x == 0) a.desc[blockIdx.x].z = 0;
@@ -781,69 +784,86 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   }
 }
 
-// Joins the pieces of the items that several CTAs hold: block (c, r) takes
-// head r of the item that starts in CTA c.  All threads find the pieces'
-// weights, then groups of head_dim / 4 threads share the pieces out.
+// Joins the pieces of the items that several CTAs hold: block (c, y) takes
+// `heads` heads of the item that starts in CTA c.  All threads find the pieces'
+// weights, then groups of heads head_dim / 4 threads share the pieces out.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeMost = 1024;  // pieces of an item: the CTAs of a grid
 
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a, int heads) {
+  grid_dep_wait();  // (launched as the decode kernel drains)
   const int4 d = a.desc[blockIdx.x];
   if (d.z == 0) return;
   int h0, nr;
   block_heads(a, d.y, h0, nr);
-  const int r = blockIdx.y;
-  if (r >= nr) return;
-  __shared__ float red[2][kMergeThreads / 32], w[kMergeMost];
+  const int r0 = blockIdx.y * heads;
+  if (r0 >= nr) return;
+  heads = min(heads, nr - r0);
+  __shared__ float w[kMergeMost * 8], total[8], top[8];
   __shared__ float4 so[kMergeThreads];
-  const int STATE = state_floats(a.hd), hd = a.hd, M0 = 8 * hd + r, L0 = 8 * hd + 8 + r;
+  const int STATE = state_floats(a.hd), hd = a.hd, M0 = 8 * hd + r0, L0 = 8 * hd + 8 + r0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // (the first CTA's piece is its second slot)
   const float* base = a.part + (size_t)blockIdx.x * 2 * STATE;
   auto piece = [&](int k) { return base + ((size_t)k * 2 + (k == 0 ? 1 : 0)) * STATE; };
-  float M = -INFINITY;
-  for (int k = tid; k < d.z; k += kMergeThreads) {
-    w[k] = piece(k)[M0];
-    M = fmaxf(M, w[k]);
+  // warp r: the pieces' weights of head r0 + r
+  if (warp < heads) {
+    float M = -INFINITY;
+    for (int k = lane; k < d.z; k += 32) {
+      const float m = piece(k)[M0 + warp];
+      w[k * heads + warp] = m;
+      M = fmaxf(M, m);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = ref_of(M);
+    float l = 0.f;
+    for (int k = lane; k < d.z; k += 32) {
+      const float x = ex2(w[k * heads + warp] - ref);
+      w[k * heads + warp] = x;
+      l = fmaf(x, piece(k)[L0 + warp], l);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      total[warp] = l;
+      top[warp] = M;
+    }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) red[0][warp] = M;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kMergeThreads / 32; ++i) M = fmaxf(M, red[0][i]);
-  const float ref = ref_of(M);
-  float l = 0.f;
-  for (int k = tid; k < d.z; k += kMergeThreads) {
-    w[k] = ex2(w[k] - ref);
-    l += w[k] * piece(k)[L0];
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  const int per = hd / 4, groups = kMergeThreads / per, x = tid % per, grp = tid / per;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int per = heads * hd / 4, groups = max(1, kMergeThreads / per);  // (per may exceed the block: 8 heads of 128)
+  const int64_t row = (int64_t)d.x * a.H + h0 + r0;
+  for (int x0 = 0; x0 < per; x0 += kMergeThreads) {
+    const int x = x0 + tid % min(per, kMergeThreads), grp = groups > 1 ? tid / per : 0, r = 4 * x / hd;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp < groups && x < per) {
 #pragma unroll 4
-  for (int k = grp; k < d.z; k += groups) {
-    const float4 v = *reinterpret_cast<const float4*>(piece(k) + r * hd + 4 * x);
-    o.x = fmaf(w[k], v.x, o.x);
-    o.y = fmaf(w[k], v.y, o.y);
-    o.z = fmaf(w[k], v.z, o.z);
-    o.w = fmaf(w[k], v.w, o.w);
-  }
-  so[tid] = o;
-  __syncthreads();
-  if (tid < hd) {
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMergeThreads / 32; ++i) l += red[1][i];
-    const float* col = reinterpret_cast<const float*>(so) + tid;
-    float sum = 0.f;
-    for (int k = 0; k < groups; ++k) sum += col[k * hd];
-    const int64_t row = (int64_t)d.x * a.H + h0 + r;
-    a.out[row * hd + tid] = a.state ? sum : (l == 0.f ? 0.f : sum / l);
-    if (a.state && tid == 0) *reinterpret_cast<float2*>(a.state + row * 2) = make_float2(M, l);
+      for (int k = grp; k < d.z; k += groups) {
+        const float4 v = *reinterpret_cast<const float4*>(piece(k) + r0 * hd + 4 * x);
+        const float p = w[k * heads + r];
+        o.x = fmaf(p, v.x, o.x);
+        o.y = fmaf(p, v.y, o.y);
+        o.z = fmaf(p, v.z, o.z);
+        o.w = fmaf(p, v.w, o.w);
+      }
+    }
+    if (groups > 1) {
+      so[tid] = o;
+      __syncthreads();
+      if (grp == 0)
+        for (int k = 1; k < groups; ++k) {
+          const float4 v = so[k * per + tid];
+          o.x += v.x;
+          o.y += v.y;
+          o.z += v.z;
+          o.w += v.w;
+        }
+    }
+    if (grp == 0 && x < per) {
+      const float l = total[r], inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      *reinterpret_cast<float4*>(a.out + row * hd + 4 * x) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      if (a.state && 4 * x == r * hd) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(top[r], l);
+    }
   }
 }
 
@@ -930,8 +950,20 @@ static int32_t launch(DecodeArgs a, cudaStream_t st) {
   const int grid = (int)std::min<int64_t>(std::min(sm_count() * S::CTAS, kMergeMost), most);
   kern<<<grid, kDecodeThreads, smem, st>>>(a, maps);
   Q6W_LAUNCH_CHECK("decode_kernel");
-  merge_kernel<<<dim3(grid, std::min(8, a.F > 1 ? a.F * a.b.rep : a.per)), kMergeThreads, 0, st>>>(a);
-  Q6W_LAUNCH_CHECK("merge_kernel");
+  // An item of few pieces is joined by one block, its heads together; where there
+  // are fewer items than CTAs an item has many pieces: a block a head.
+  const int nr = a.F > 1 ? a.F * a.b.rep : a.per;
+  const int heads = (int64_t)a.b.n * (a.b.kv_heads / a.F) * a.HB >= grid ? nr : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)((nr + heads - 1) / heads));
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  Q6W_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_kernel, a, heads));
   return Q6W_OK;
 }
 
