@@ -85,7 +85,7 @@ struct TcShape {
   static constexpr int REGS = 128;
   static constexpr int SOFT_REGS = kHalf ? 168 : 152, LOAD_REGS = kHalf ? 104 : 136, MMA_REGS = 72;
   static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
-  static constexpr int kFlush = kHalf ? 4 : 1;  // units between additions of O to registers
+  static constexpr int kFlush = kHalf ? 4 : 2;  // units between additions of O to registers
   static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
 };
 
@@ -733,6 +733,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     constexpr int NCH = KEYS / 32 / HALVES;    // 32-key chunks of a unit that this thread takes
     constexpr int MYD = HD / HALVES;           // dims of O that this thread takes
     const int ch0 = hf * NCH;
+    constexpr int DW = MYD < 32 ? 16 : 32;     // dims of O read at a time
     // With two threads a row, a warp and its partner (the same rows' other half)
     // pass the same barriers: both see the same verdict and stop together.
     auto agree = [&](bool mine) -> bool {
@@ -856,11 +857,11 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         if (uu > 0 && (flush || grow)) before();
         if (flush) {
 #pragma unroll
-          for (int d = 0; d < MYD; d += 16) {
-            float v[16];
+          for (int d = 0; d < MYD; d += DW) {
+            float v[DW];
             tmem_load(ocol + d, v);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[d + e] += v[e];
+            for (int e = 0; e < DW; ++e) acc[d + e] += v[e];
           }
         }
         if (grow) {
