@@ -620,3 +620,37 @@ def test_model_step_from_ops_matches_the_cached_step(tmp_path_factory, kv, prefi
         got = forward(tok[t], table, lengths, None, prefix)
         want, _ = model.forward_batch(tok[t].int(), lengths + (prefix - 1), kc, vc)
         assert (got - want).abs().max() <= 4e-4
+
+
+# ---- refusals of the Python operators ------------------------------------------------------
+
+
+def test_python_refusals():
+    c = make(3, 8, 2, 64, 16, torch.float32, [3, 20, 8], [1, 1, 1])
+    a = dict(queries=c["q"], key_pages=c["kp"], value_pages=c["vp"], page_table=c["table"], lengths=c["lens"])
+    bad = [dict(queries=c["q"].half()), dict(queries=c["q"][:, :, :32]), dict(queries=c["q"].transpose(1, 2)),
+           dict(queries=c["q"][:2]), dict(key_pages=c["kp"].half()), dict(key_pages=c["kp"].double()),
+           dict(key_pages=c["kp"][:-1]), dict(value_pages=c["vp"].transpose(1, 2).contiguous().transpose(1, 2)),
+           dict(page_table=c["table"].long()), dict(page_table=c["table"].t().contiguous().t()), dict(page_table=c["table"][0]),
+           dict(lengths=c["lens"].long()), dict(lengths=c["lens"][:2]), dict(lengths=c["lens"].cpu()),
+           dict(query_starts=c["starts"][:3]), dict(query_starts=c["starts"].long()),
+           dict(status=torch.zeros(1, device="cuda")), dict(out=torch.empty(3, 8, 32, device="cuda")),
+           dict(out=torch.empty(3, 8, 128, device="cuda")[:, :, ::2])]
+    ops.paged_attention(**a)
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.paged_attention(**{**a, **kw})
+    with pytest.raises(Q6WError):  # seven heads over two kv heads
+        ops.paged_attention(**{**a, "queries": c["q"][:, :7].contiguous()})
+    pages = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for length in (-1, 33):
+        with pytest.raises(ValueError):
+            ops.shared_prefix_attention(prefix_pages=pages, prefix_length=length, **a)
+    cos, sin = tables(64, 64)
+    q, k, v = append_inputs(3, 8, 2, 64, 1)
+    b = dict(a, queries=q, keys=k, values=v, cos=cos, sin=sin)
+    ops.paged_append(**b)
+    for kw in (dict(keys=k[:, :1]), dict(keys=k[:2]), dict(values=v[:2]), dict(values=v.half()), dict(cos=cos[:, :16]),
+               dict(sin=sin[:5]), dict(cos=cos.double(), sin=sin.double()), dict(queries=q[:2]), dict(out=q)):
+        with pytest.raises(ValueError):
+            ops.paged_append(**{**b, **kw})

@@ -119,12 +119,6 @@ struct DecodeMaps {
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 
-// a b / c, in 32 bits when the product fits (a 64-bit division is a long subroutine).
-__device__ __forceinline__ int64_t muldiv(int64_t a, int64_t b, int64_t c) {
-  const int64_t p = a * b;
-  return (p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)c) : p / c;
-}
-
 // The line of units: prefix sums over 256 stretches of sequences.
 struct Line {
   int64_t pref[kDecodeThreads];

@@ -266,9 +266,9 @@ struct Walk {
     if (a.prefix) {
       sequence();
       const int per = max(1, (a.prefix_len + KEYS - 1) / KEYS), nb = blocks();
-      p.kv = (int)(rem / ((int64_t)per * nb));
+      p.kv = (int)muldiv(rem, 1, (int64_t)per * nb);
       rem -= (int64_t)p.kv * per * nb;
-      p.j = (int)(rem / per);
+      p.j = (int)muldiv(rem, 1, per);
       rem -= (int64_t)p.j * per;
       block();
     } else {
@@ -281,7 +281,7 @@ struct Walk {
       rem -= a.line[lo] * a.b.kv_heads;
       sequence();
       const int64_t per = a.line[lo + 1] - a.line[lo];
-      p.kv = (int)(rem / per);
+      p.kv = (int)muldiv(rem, 1, per);
       rem -= p.kv * per;
       for (p.j = 0;; ++p.j) {
         block();
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   const int64_t c = blockIdx.x;
   Walk<S::ROWS, KEYS> w(a);
   if (c < workers)
-    w.begin(c * units / workers, (c + 1) * units / workers);
+    w.begin(muldiv(c, units, workers), muldiv(c + 1, units, workers));
   else
     w.begin(0, 0);
   const int64_t x0 = w.p.x;
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           down = __uint_as_float((uint32_t)(254 - ex) << 23);
           sc *= __uint_as_float((uint32_t)ex << 23);
         }
-#pragma unroll 1
+#pragma unroll 2
         for (int e0 = hf * MYD; e0 < (hf + 1) * MYD; e0 += 16) {
           uint32_t part[QP][8];
 #pragma unroll
@@ -979,42 +979,62 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   }
 }
 
-// Joins the pieces of blocks that several CTAs hold: block (c, y) takes 16 rows
-// of the item that starts in CTA c, a warp a row at a time.
+// Sum of `pieces` partial states of a row and, with `own`, the state that its
+// place in `out` holds; by one warp: groups of HD / 4 lanes take every
+// 32 / (HD / 4)-th piece, four dims a lane.  at(k): the row's index in part.
+template <int HD, typename At>
+__device__ __forceinline__ void join_row(const TcArgs& a, int64_t row, int pieces, bool own, const At& at, int lane) {
+  constexpr int W = HD / 4, G = 32 / W;
+  const int x = lane % W, g = lane / W;
+  const float m0 = own ? a.state[row * 2] : -INFINITY;
+  float M = m0;
+  for (int k = lane; k < pieces; k += 32) M = fmaxf(M, a.part_ml[at(k) * 2]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = ref_of(M);
+  float l = 0.f;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m, float li, const float* o) {
+    const float w = ex2(m - ref);
+    const float4 v = *reinterpret_cast<const float4*>(o + 4 * x);
+    l = fmaf(w, li, l);
+    s.x = fmaf(w, v.x, s.x);
+    s.y = fmaf(w, v.y, s.y);
+    s.z = fmaf(w, v.z, s.z);
+    s.w = fmaf(w, v.w, s.w);
+  };
+  if (own && g == 0) add(m0, a.state[row * 2 + 1], a.out + row * HD);
+#pragma unroll 4
+  for (int k = g; k < pieces; k += G) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(k) * 2);
+    add(ml.x, ml.y, a.part + at(k) * HD);
+  }
+#pragma unroll
+  for (int o = W; o < 32; o <<= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, o);
+    s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+    s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+    s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+  }
+  const bool state = a.state && !own;  // the state itself, to be joined with the prefix's
+  const float inv = state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+  if (g == 0) *reinterpret_cast<float4*>(a.out + row * HD + 4 * x) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+  if (state && lane == 0) *reinterpret_cast<float2*>(a.state + row * 2) = make_float2(M, l);
+}
+
+// Joins the pieces of blocks that several CTAs hold: block (c, y) takes 8 rows
+// of the item that starts in CTA c, a warp a row.
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(128) rows_merge_kernel(TcArgs a) {
+__global__ void __launch_bounds__(256) rows_merge_kernel(TcArgs a) {
   const int c = blockIdx.x;
   const int4 d = a.desc[2 * c];
   if (d.w == 0) return;
-  const int rows = a.desc[2 * c + 1].x, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < 16; i += 4) {
-    const int r = blockIdx.y * 16 + i;
-    if (r >= rows) return;
-    auto at = [&](int k) { return (int64_t)((c + k) * 2 + (k == 0 ? 1 : 0)) * ROWS + r; };
-    float M = -INFINITY;
-    for (int k = lane; k < d.w; k += 32) M = fmaxf(M, a.part_ml[at(k) * 2]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = ref_of(M);
-    float l = 0.f, acc[(HD + 31) / 32] = {};
-    for (int k = 0; k < d.w; ++k) {
-      const float w = ex2(a.part_ml[at(k) * 2] - ref);
-      l += w * a.part_ml[at(k) * 2 + 1];
-#pragma unroll
-      for (int x = 0; x < (HD + 31) / 32; ++x)
-        if (x * 32 + lane < HD) acc[x] = fmaf(w, a.part[at(k) * HD + x * 32 + lane], acc[x]);
-    }
-    const int ri = d.z * ROWS + r, tok = ri / a.b.rep, h = d.y * a.b.rep + ri - tok * a.b.rep;
-    const int64_t row = (int64_t)(d.x + tok) * a.H + h;
-    const float inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-#pragma unroll
-    for (int x = 0; x < (HD + 31) / 32; ++x)
-      if (x * 32 + lane < HD) a.out[row * HD + x * 32 + lane] = acc[x] * inv;
-    if (a.state && lane == 0) {
-      a.state[row * 2] = M;
-      a.state[row * 2 + 1] = l;
-    }
-  }
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= a.desc[2 * c + 1].x) return;
+  const int ri = d.z * ROWS + r, tok = ri / a.b.rep, h = d.y * a.b.rep + ri - tok * a.b.rep;
+  join_row<HD>(a, (int64_t)(d.x + tok) * a.H + h, d.w, false,
+               [&](int k) { return (int64_t)((c + k) * 2 + (k == 0 ? 1 : 0)) * ROWS + r; }, threadIdx.x & 31);
 }
 
 // Zeros the rows of tokens that no sequence holds.
@@ -1044,28 +1064,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(TcArgs a, int64_t unit
   const int64_t item = (int64_t)kv * (a.items / a.b.kv_heads) + j;
   const int64_t c0 = owner_of(item * per, units, workers);
   const int pieces = (int)(owner_of(item * per + per - 1, units, workers) - c0) + 1;
-  auto at = [&](int k) { return ((int64_t)k * a.items + item) * ROWS + (ri - j * ROWS); };
-  const float m0 = a.state[row * 2];
-  float M = m0;
-  for (int k = lane; k < pieces; k += 32) M = fmaxf(M, a.part_ml[at(k) * 2]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float ref = ref_of(M);
-  float w = ex2(m0 - ref), l = w * a.state[row * 2 + 1], acc[(HD + 31) / 32];
-#pragma unroll
-  for (int x = 0; x < (HD + 31) / 32; ++x) acc[x] = x * 32 + lane < HD ? w * a.out[row * HD + x * 32 + lane] : 0.f;
-#pragma unroll 4
-  for (int k = 0; k < pieces; ++k) {
-    w = ex2(a.part_ml[at(k) * 2] - ref);
-    l += w * a.part_ml[at(k) * 2 + 1];
-#pragma unroll
-    for (int x = 0; x < (HD + 31) / 32; ++x)
-      if (x * 32 + lane < HD) acc[x] = fmaf(w, a.part[at(k) * HD + x * 32 + lane], acc[x]);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int x = 0; x < (HD + 31) / 32; ++x)
-    if (x * 32 + lane < HD) a.out[row * HD + x * 32 + lane] = acc[x] * inv;
+  join_row<HD>(a, row, pieces, true, [&](int k) { return ((int64_t)k * a.items + item) * ROWS + (ri - j * ROWS); }, lane);
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -1113,7 +1112,7 @@ struct TcLaunch {
     Q6W_LAUNCH_CHECK("line_kernel");
     int32_t rc = rows(a, st);
     if (rc) return rc;
-    rows_merge_kernel<HD, S::ROWS><<<dim3(sm_count(), S::ROWS / 16), 128, 0, st>>>(a);
+    rows_merge_kernel<HD, S::ROWS><<<dim3(sm_count(), S::ROWS / 8), 256, 0, st>>>(a);
     Q6W_LAUNCH_CHECK("rows_merge_kernel");
     return Q6W_OK;
   }
