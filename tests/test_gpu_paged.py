@@ -192,6 +192,30 @@ def test_append_many_sequences_finds_each_token():
     assert torch.equal(got, rotated(q, cos[pos][:, None], sin[pos][:, None]))
 
 
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+def test_append_many_tokens(kv):
+    """Enough narrow tokens that a thread takes several, across the ends of
+    sequences, with empty sequences and padding at both ends and inside."""
+    g = torch.Generator().manual_seed(8)
+    n = 600
+    new = torch.randint(0, 41, (n,), generator=g)
+    new[50:60] = 0
+    c = make(n, 8, 4, 16, 16, kv, torch.randint(0, 30, (n,), generator=g).tolist(), new.tolist())
+    T = int(new.sum())
+    assert T * 32 >= 148 * 2048
+    c["past"][7] -= int(c["past"][7]) + 3  # the first three new tokens of sequence 7 are padding
+    c["lens"][7] = c["past"][7] + int(new[7])
+    cos, sin = tables(128, 16)
+    q, k, v = append_inputs(T + 9, 8, 4, 16, 12)
+    kp, vp, pos = expected_pools(c, k[4:], v[4:], cos, sin)
+    c["starts"] += 4
+    got = ops.paged_append(q, k, v, cos, sin, c["kp"], c["vp"], c["table"], c["lens"], c["starts"])
+    assert torch.equal(c["kp"], kp) and torch.equal(c["vp"], vp)
+    pos = torch.tensor(pos).cuda()
+    want = rotated(q[4: T + 4], cos[pos.clamp(min=0)][:, None], sin[pos.clamp(min=0)][:, None]) * (pos >= 0)[:, None, None]
+    assert torch.equal(got[4: T + 4], want) and not got[:4].any() and not got[T + 4:].any()
+
+
 def test_append_padding_rows():
     """Tokens in front of the first sequence, behind the last, and in front of
     position 0 append nothing; their rows stay as they were or come back zero."""

@@ -16,6 +16,8 @@ namespace paged {
 // that the search for the token's sequence is a warp's), eight consecutive
 // elements a thread and step: two 16-byte loads, one or two 16-byte stores.
 
+constexpr int kGroup = 4;  // tokens of a thread, narrow tokens
+
 struct AppendArgs {
   Batch b;
   const float* q;
@@ -41,62 +43,111 @@ __device__ __forceinline__ void store8(void* pool, int64_t off, int half, const 
   }
 }
 
+// A token's place: its sequence's index of it, position, page slot.
+struct Place {
+  int at;         // index among the sequence's own tokens; out of range: nothing is written
+  int64_t pos;    // position of the rotation
+  int64_t slot;   // element offset of the slot, -1: a bad page id
+  bool in;
+};
+
+// Sequence s holds tokens [t0, t1); moves on to the one that holds t.
+__device__ __forceinline__ void follow(const Batch& b, int t, int& s, int& t0, int& t1) {
+  while (s < b.n && t >= t1) {
+    if (++s < b.n) seq_tokens(b, s, t0, t1);
+  }
+}
+
+__device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int s, int t0, int t1) {
+  const Batch& b = a.b;
+  Place p;
+  p.at = s >= 0 && s < b.n && t >= t0 && t < t1 ? seq_length(b, s) - (t1 - t) : -1;
+  p.pos = (int64_t)a.first + p.at;
+  p.in = p.at >= 0 && p.at < b.max_len && p.pos < a.rope_len;
+  p.slot = -1;
+  if (p.in) {
+    const int page = __ldg(b.table + s * b.table_stride + (p.at >> b.shift));
+    if ((unsigned)page < (unsigned)b.n_pages)
+      p.slot = page * b.page_stride + (int64_t)(p.at & ((1 << b.shift) - 1)) * b.slot_stride;
+  }
+  if (p.at >= 0 && p.slot < 0) flag(b.status, kErrInput);
+  return p;
+}
+
+struct Unit {
+  float x[8];
+};
+
+__device__ __forceinline__ Unit load_unit(const AppendArgs& a, int t, int i, int nq, int nk) {
+  const float* src = i < nq        ? a.q + t * a.ldq + 8 * i
+                     : i < nq + nk ? a.k + t * a.ldk + 8 * (i - nq)
+                                   : a.v + t * a.ldv + 8 * (i - nq - nk);
+  const float4 lo = __ldcs(reinterpret_cast<const float4*>(src));
+  const float4 hi = __ldcs(reinterpret_cast<const float4*>(src) + 1);
+  return {{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}};
+}
+
+// Rotates (queries, keys) and stores unit i of token t.
 template <bool HALF>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int tpt = 1 << a.tpt_shift;
-  const int t = blockIdx.x * (256 >> a.tpt_shift) + (threadIdx.x >> a.tpt_shift);
-  if (t >= a.b.T) return;  // warp-uniform: tpt >= 32
-  const int s = token_seq(a.b, t, lane);
-  int at = -1;  // index among the sequence's own tokens
-  if (s >= 0 && s < a.b.n) {
-    int t0, t1;
-    seq_tokens(a.b, s, t0, t1);
-    at = seq_length(a.b, s) - (t1 - t);
-  }
-  const int64_t pos = (int64_t)a.first + at;
-  if (at < 0 || at >= a.b.max_len || pos >= a.rope_len) {
-    if (at >= 0) flag(a.b.status, kErrInput);
-    if (a.zero)
-      for (int i = threadIdx.x & (tpt - 1); i < a.H * (a.hd >> 2); i += tpt)
-        reinterpret_cast<float4*>(a.out + (int64_t)t * a.H * a.hd)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    return;
-  }
-  const int page = __ldg(a.b.table + s * a.b.table_stride + (at >> a.b.shift));
-  const bool page_ok = page >= 0 && page < a.b.n_pages;
-  if (!page_ok) flag(a.b.status, kErrInput);
-  const int64_t slot = page * a.b.page_stride + (int64_t)(at & ((1 << a.b.shift) - 1)) * a.b.slot_stride;
-  const int hd = a.hd, units = hd >> 3;  // eight-element units of a head
-  const int nq = a.H * units, nk = a.b.kv_heads * units;
-  const float* cs = a.cs + pos * (hd >> 1);
-  const float* sn = a.sn + pos * (hd >> 1);
-  for (int i = threadIdx.x & (tpt - 1); i < nq + 2 * nk; i += tpt) {
-    const float* src;
-    const int j = i < nq ? i : (i < nq + nk ? i - nq : i - nq - nk);
-    if (i < nq)
-      src = a.q + t * a.ldq + 8 * j;
-    else
-      src = (i < nq + nk ? a.k + t * a.ldk : a.v + t * a.ldv) + 8 * j;
-    const float4 lo = __ldcs(reinterpret_cast<const float4*>(src));
-    const float4 hi = __ldcs(reinterpret_cast<const float4*>(src) + 1);
-    float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    const int u = j % units;
-    if (i < nq + nk) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(cs + 4 * u));
-      const float4 d = __ldg(reinterpret_cast<const float4*>(sn + 4 * u));
-      const float cc[4] = {c.x, c.y, c.z, c.w}, dd[4] = {d.x, d.y, d.z, d.w};
+__device__ __forceinline__ void finish_unit(const AppendArgs& a, int t, int i, int nq, int nk, const Place& p, Unit& v) {
+  const int units = a.hd >> 3;
+  const int j = i < nq ? i : (i < nq + nk ? i - nq : i - nq - nk);
+  const int u = j & (units - 1);
+  float(&x)[8] = v.x;
+  if (!p.in) {
+    if (i >= nq || !a.zero) return;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float x0 = x[2 * p], x1 = x[2 * p + 1];
-        x[2 * p] = __fsub_rn(__fmul_rn(x0, cc[p]), __fmul_rn(x1, dd[p]));
-        x[2 * p + 1] = __fadd_rn(__fmul_rn(x0, dd[p]), __fmul_rn(x1, cc[p]));
-      }
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  } else if (i < nq + nk) {
+    const float4 c = __ldg(reinterpret_cast<const float4*>(a.cs + p.pos * (a.hd >> 1) + 4 * u));
+    const float4 d = __ldg(reinterpret_cast<const float4*>(a.sn + p.pos * (a.hd >> 1) + 4 * u));
+    const float cc[4] = {c.x, c.y, c.z, c.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x0 = x[2 * e], x1 = x[2 * e + 1];
+      x[2 * e] = __fsub_rn(__fmul_rn(x0, cc[e]), __fmul_rn(x1, dd[e]));
+      x[2 * e + 1] = __fadd_rn(__fmul_rn(x0, dd[e]), __fmul_rn(x1, cc[e]));
     }
-    if (i < nq) {
-      store8(a.out, ((int64_t)t * a.H) * hd + 8 * j, 0, x);
-    } else if (page_ok) {
-      const int64_t off = slot + (j / units) * a.b.head_stride + 8 * u;
-      store8(i < nq + nk ? a.b.k : a.b.v, off, HALF, x);
+  }
+  if (i < nq)
+    store8(a.out, ((int64_t)t * a.H) * a.hd + 8 * j, 0, x);
+  else if (p.slot >= 0)
+    store8(i < nq + nk ? a.b.k : a.b.v, p.slot + (int64_t)(j / units) * a.b.head_stride + 8 * u, HALF, x);
+}
+
+// GROUP tokens a thread: where one step of tpt threads covers a token, several
+// (their loads go first, in flight together, and one search serves them); wide
+// tokens one, its units one ahead.
+template <bool HALF, int GROUP>
+__global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int tpt = 1 << a.tpt_shift, me = threadIdx.x & (tpt - 1);
+  const int t = (blockIdx.x * (256 >> a.tpt_shift) + (threadIdx.x >> a.tpt_shift)) * GROUP;
+  if (t >= a.b.T) return;  // warp-uniform: tpt >= 32
+  const int units = a.hd >> 3;  // eight-element units of a head
+  const int nq = a.H * units, nk = a.b.kv_heads * units, all = nq + 2 * nk;
+  Unit x[GROUP];
+#pragma unroll
+  for (int g = 0; g < GROUP; ++g)
+    if (me < all && t + g < a.b.T) x[g] = load_unit(a, t + g, me, nq, nk);
+  int s = token_seq(a.b, t, lane), t0 = 0, t1 = 0;
+  if (s >= 0 && s < a.b.n) seq_tokens(a.b, s, t0, t1);
+  if (GROUP > 1) {
+#pragma unroll
+    for (int g = 0; g < GROUP; ++g) {
+      if (t + g >= a.b.T) break;
+      if (g > 0) follow(a.b, t + g, s, t0, t1);
+      const Place p = place_of(a, t + g, s, t0, t1);
+      if (me < all) finish_unit<HALF>(a, t + g, me, nq, nk, p, x[g]);
+    }
+  } else {
+    const Place p = place_of(a, t, s, t0, t1);
+    for (int i = me; i < all;) {
+      Unit v = x[0];
+      const int cur = i;
+      i += tpt;
+      if (i < all) x[0] = load_unit(a, t, i, nq, nk);
+      finish_unit<HALF>(a, t, cur, nq, nk, p, v);
     }
   }
 }
@@ -320,12 +371,15 @@ extern "C" int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_toke
   const int units = (n_heads + 2 * batch->kv_heads) * (batch->head_dim >> 3);
   a.tpt_shift = 5;
   while (a.tpt_shift < 8 && (1 << a.tpt_shift) < units) ++a.tpt_shift;
-  const int per = 256 >> a.tpt_shift;
+  // kGroup tokens a thread where a token is one step of its threads and the GPU
+  // stays full; else one.
+  const bool many = units <= 256 && (int64_t)n_tokens << a.tpt_shift >= (int64_t)sm_count() * 2048;
+  const int per = (256 >> a.tpt_shift) * (many ? paged::kGroup : 1);
   const unsigned grid = (unsigned)((n_tokens + per - 1) / per);
-  if (batch->kv_dtype == Q6W_KV_F16)
-    paged::append_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-  else
-    paged::append_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+  const bool half = batch->kv_dtype == Q6W_KV_F16;
+  auto kern = many ? (half ? paged::append_kernel<true, paged::kGroup> : paged::append_kernel<false, paged::kGroup>)
+                   : (half ? paged::append_kernel<true, 1> : paged::append_kernel<false, 1>);
+  kern<<<grid, 256, 0, (cudaStream_t)stream>>>(a);
   Q6W_LAUNCH_CHECK("append_kernel");
   return Q6W_OK;
 }
