@@ -439,6 +439,34 @@ def test_length_beyond_the_table_is_flagged():
     ops.check_status(status)
 
 
+def test_padding_inside_ragged_sequences():
+    """More new tokens than a sequence's length: the first ones are padding (zero
+    rows), the others as in a call that holds them alone."""
+    for prefix in (0, 60):
+        c = make(2, 8, 2, 64, 16, torch.float16, [0, 30], [90, 20], prefix=prefix)
+        c["lens"][0] = 50  # 40 of the 90 are padding
+        got = attend(c)
+        d = dict(c, q=c["q"][40:].contiguous(), new=[50, 20], past=[0, 30])
+        d["starts"] = torch.tensor([0, 50, 70], dtype=torch.int32).cuda()
+        check(d, got[40:])
+        if not prefix:
+            assert not got[:40].any()
+        else:  # they see the prefix alone
+            k, v = (x[c["prefix_pages"].long()].flatten(0, 1)[:60].double() for x in (c["kp"], c["vp"]))
+            w = torch.softmax(torch.einsum("tgrd,kgd->tgrk", c["q"][:40].double().unflatten(1, (2, 4)), k) / 8, -1)
+            want = torch.einsum("tgrk,kgd->tgrd", w, v).flatten(1, 2)
+            assert (got[:40].double() - want).abs().max() <= 300 * U * float(v.abs().max())
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+def test_decode_one_long_among_many(kv):
+    """A request that reaches over most of the GPU among many that fill a tile each."""
+    past = [3] * 700
+    past[350] = 60000
+    c = make(700, 16, 2, 64, 16, kv, past, [1] * 700, seed=4)
+    check(c, attend(c))
+
+
 def test_rows_outside_the_sequences():
     c = make(2, 8, 4, 16, 16, torch.float32, [3, 30], [4, 10])
     want = attend(c)

@@ -778,21 +778,24 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   }
 }
 
-// Joins the pieces of the items that several CTAs hold: block (c, y) takes
-// `heads` heads of the item that starts in CTA c.  All threads find the pieces'
-// weights, then groups of heads head_dim / 4 threads share the pieces out.
+// Joins the pieces of the items that several CTAs hold: block (c, 0) all heads of
+// the item that starts in CTA c when it has few pieces (8192 short requests: 12 us
+// with a block a head, 5 so), block (c, y) head y when it has many (one long request:
+// a block for all would walk over 111 pieces of 512 floats).  A warp a head finds the
+// pieces' weights, then groups of heads head_dim / 4 threads share the pieces out.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeMost = 1024;  // pieces of an item: the CTAs of a grid
 
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a, int heads) {
+constexpr int kFewPieces = 8;
+
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
   grid_dep_wait();  // (launched as the decode kernel drains)
   const int4 d = a.desc[blockIdx.x];
   if (d.z == 0) return;
   int h0, nr;
   block_heads(a, d.y, h0, nr);
-  const int r0 = blockIdx.y * heads;
-  if (r0 >= nr) return;
-  heads = min(heads, nr - r0);
+  const int r0 = blockIdx.y, heads = d.z <= kFewPieces ? nr : 1;
+  if (r0 >= nr || (heads > 1 && r0 > 0)) return;
   __shared__ float w[kMergeMost * 8], total[8], top[8];
   __shared__ float4 so[kMergeThreads];
   const int STATE = state_floats(a.hd), hd = a.hd, M0 = 8 * hd + r0, L0 = 8 * hd + 8 + r0;
@@ -944,12 +947,8 @@ static int32_t launch(DecodeArgs a, cudaStream_t st) {
   const int grid = (int)std::min<int64_t>(std::min(sm_count() * S::CTAS, kMergeMost), most);
   kern<<<grid, kDecodeThreads, smem, st>>>(a, maps);
   Q6W_LAUNCH_CHECK("decode_kernel");
-  // An item of few pieces is joined by one block, its heads together; where there
-  // are fewer items than CTAs an item has many pieces: a block a head.
-  const int nr = a.F > 1 ? a.F * a.b.rep : a.per;
-  const int heads = (int64_t)a.b.n * (a.b.kv_heads / a.F) * a.HB >= grid ? nr : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid, (unsigned)((nr + heads - 1) / heads));
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)(a.F > 1 ? a.F * a.b.rep : a.per));
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -957,7 +956,7 @@ static int32_t launch(DecodeArgs a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  Q6W_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_kernel, a, heads));
+  Q6W_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_kernel, a));
   return Q6W_OK;
 }
 
