@@ -83,7 +83,7 @@ struct TcShape {
   // (what the block was launched with, 64 K / THREADS a thread, divided anew).
   static constexpr int THREADS = 32 * (SOFT + 8);
   static constexpr int REGS = 128;
-  static constexpr int SOFT_REGS = kHalf ? 168 : 152, LOAD_REGS = kHalf ? 104 : 136, MMA_REGS = 72;
+  static constexpr int SOFT_REGS = 160, LOAD_REGS = 96, MMA_REGS = 96;
   static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
   static constexpr int kFlush = kHalf ? 4 : 2;  // units between additions of O to registers
   static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     int i = 0;
     bool ok = true;
     // Units through registers, BATCH loads of keys and values a thread at a time.
-    constexpr int MOST = kHalf ? 4 : 8, BATCH = NL < MOST ? NL : MOST;
+    constexpr int MOST = kHalf ? 4 : 2, BATCH = NL < MOST ? NL : MOST;
     uint4 rv[BATCH], rk[BATCH];
     int ids[BATCH];  // page ids of the batch to fetch
     auto pages = [&](const Piece& p, int u, int n0) {
