@@ -36,6 +36,12 @@
 // balance alike.  A warp that holds an item whole writes its output; pieces
 // of an item go through the workspace, joined by their CTA when it holds them
 // all, else by merge_kernel.
+//
+// Measured (a call, joins included): 64 requests of 128-16384 keys, FP16, 8 heads a
+// group of 64: 102-107 us for 542 MB, 5.1-5.3 TB/s; 37 requests, FP32, 5 heads a group of
+// 128: 85 us for 380 MB; 8192 requests of 20-147 keys, FP32, heads of 16: 94 us for 357 MB,
+// bound by instruction issue; one request of 32768 keys, FP32: 27 us for 67 MB, of
+// which start-up and joins are about 15.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -779,8 +785,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
 }
 
 // Joins the pieces of the items that several CTAs hold: block (c, 0) all heads of
-// the item that starts in CTA c when it has few pieces (8192 short requests: 12 us
-// with a block a head, 5 so), block (c, y) head y when it has many (one long request:
+// the item that starts in CTA c when it has few pieces (8192 short requests: 11.7 us
+// with a block a head, 5.9 so), block (c, y) head y when it has many (one long request:
 // a block for all would walk over 111 pieces of 512 floats).  A warp a head finds the
 // pieces' weights, then groups of heads head_dim / 4 threads share the pieces out.
 constexpr int kMergeThreads = 256;
