@@ -12,6 +12,7 @@
 
 #include "async.cuh"
 #include "common.cuh"
+#include "share.cuh"
 
 namespace q6w {
 namespace paged {
@@ -82,18 +83,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
-
-// a b / c, in 32 bits when the product fits (a 64-bit division is a long subroutine).
-__device__ __forceinline__ int64_t muldiv(int64_t a, int64_t b, int64_t c) {
-  const int64_t p = a * b;
-  return (p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)c) : p / c;
-}
-
-// Worker w holds units [w units / workers, (w + 1) units / workers): the one that holds `unit`.
-__device__ __forceinline__ int64_t owner_of(int64_t unit, int64_t units, int64_t workers) {
-  const int64_t p = (unit + 1) * workers + units - 1;
-  return ((p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)units) : p / units) - 1;
-}
 
 // The pool's tensor map (paged_decode.cu).
 int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, int segments, CUtensorMap* map,
