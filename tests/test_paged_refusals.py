@@ -117,3 +117,14 @@ def test_python_ops_refuse_the_cpu():
         ops.paged_attention(q, pool, pool, table, lens)
     with pytest.raises(ValueError):
         ops.shared_prefix_attention(q, pool, pool, table[0], 3, table, lens)
+
+
+def test_rows_are_counted_in_32_bits():
+    """2^24 tokens of 128 heads: the row numbers of the attention kernels would wrap."""
+    many = batch(kv_heads=1, head_dim=16, slot_stride=16, page_stride=256, head_stride=16, query_starts=P)
+    for kw in (dict(), dict(prefix=P, P_len=5)):
+        assert attend(many, T=1 << 24, H=128, ldq=2048, **kw) == _lib.Q6W_ERR_ARG
+        assert "32 bits" in message()
+        # one head fewer passes this check and stops at the next one
+        assert attend(many, T=1 << 24, H=127, ldq=2048, ws=None, **kw) == _lib.Q6W_ERR_ARG
+        assert "workspace" in message()

@@ -265,6 +265,9 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
   if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
   if (p->page_size * p->head_dim * (p->kv_dtype == Q6W_KV_F16 ? 2 : 4) < 128)
     return fail(Q6W_ERR_ARG, "%s: a kv head's part of a page must be at least 128 bytes", who);
+  // row numbers, rounded up to whole tiles, are 32-bit in the kernels
+  if ((int64_t)n_tokens * n_heads > INT32_MAX - 512)
+    return fail(Q6W_ERR_ARG, "%s: %d tokens of %d heads are more rows than 32 bits count", who, n_tokens, n_heads);
   if (n_tokens == 0) return Q6W_OK;
   if (!queries || !output || (prefix_length > 0 && !prefix_pages)) return fail(Q6W_ERR_ARG, "%s: null pointer", who);
   if (!aligned(queries, 16) || !aligned(output, 16) || query_stride % 4)
