@@ -1,0 +1,64 @@
+"""GPU: waits of the paged attention kernels that run out.  With the diagnostic
+on, the first thread block waits for tiles that it never sees arrive: the call
+has to end soon, mark what it could not compute as NaN -- also where the caller
+gave no status word -- and leave everything else as it is."""
+
+import time
+
+import pytest
+import torch
+
+from q6w_b200 import Q6WError, _lib, ops
+from test_gpu_paged import attend, make
+
+pytestmark = pytest.mark.gpu
+CYCLES = 2_000_000  # about a millisecond; a tile takes a microsecond
+
+
+def stalled(c, **kw):
+    lib = _lib.load()
+    torch.cuda.synchronize()
+    _lib.check(lib.q6w_selftest_paged_stall(CYCLES))
+    try:
+        t0 = time.perf_counter()
+        out = attend(c, **kw)
+        torch.cuda.synchronize()
+        return out, time.perf_counter() - t0
+    finally:
+        _lib.check(lib.q6w_selftest_paged_stall(0))
+
+
+def check_stalled(c, heads):
+    """``heads``: (token, head) rows that surely meet the first block."""
+    want = attend(c)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for kw in (dict(status=status), dict()):
+        got, seconds = stalled(c, **kw)
+        assert seconds < 1.0
+        nan = got.isnan().any(-1)
+        assert torch.equal(nan, got.isnan().all(-1))  # whole rows
+        for t, h in heads:
+            assert bool(nan[t, h]), (t, h)
+        assert torch.equal(got[~nan], want[~nan])
+        share = float(nan.float().mean())
+    with pytest.raises(Q6WError, match="ran out of time"):
+        ops.check_status(status)
+    assert torch.equal(attend(c, status=status), want)
+    ops.check_status(status)
+    return share
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("H,KV,hd", [(8, 4, 16), (32, 4, 64), (8, 4, 128)])
+def test_decode_wait_runs_out(H, KV, hd, kv):
+    """Ragged requests: the first block holds the first ones, nobody else misses anything."""
+    c = make(2400, H, KV, hd, 16, kv, [(i * 29) % 90 for i in range(2400)], [1] * 2400, seed=3)
+    share = check_stalled(c, [(0, h) for h in range(H)])
+    assert share < 0.02
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+def test_decode_wait_runs_out_in_a_piece(kv):
+    """One long request: the first block's piece spoils the heads of the first kv head alone."""
+    c = make(1, 16, 4, 64, 16, kv, [9000], [1], seed=5)
+    assert check_stalled(c, [(0, h) for h in range(4)]) == 0.25

@@ -128,3 +128,9 @@ def test_rows_are_counted_in_32_bits():
         # one head fewer passes this check and stops at the next one
         assert attend(many, T=1 << 24, H=127, ldq=2048, ws=None, **kw) == _lib.Q6W_ERR_ARG
         assert "workspace" in message()
+
+
+def test_stall_diagnostic_arguments():
+    stall = _lib.load().q6w_selftest_paged_stall
+    assert stall(-1) == _lib.Q6W_ERR_ARG and stall((1 << 31) + 1) == _lib.Q6W_ERR_ARG
+    assert stall(0) == _lib.Q6W_OK

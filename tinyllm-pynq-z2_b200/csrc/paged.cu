@@ -2,6 +2,8 @@
 // pages, and attention of a batch behind a shared prefix.
 #include <math.h>
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace q6w {
@@ -253,6 +255,9 @@ static size_t layout(const Batch& b, int hd, int H, bool half, int prefix_length
   return s.used;
 }
 
+// Bound of the attention kernels' waits while q6w_selftest_paged_stall is on; 0: off.
+static std::atomic<int64_t> g_stall_cycles{0};
+
 static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_t* prefix_pages, int32_t prefix_length,
                          int32_t n_tokens, int32_t n_heads, const float* queries, int64_t query_stride, float* output,
                          int32_t zero_padding, void* workspace, size_t workspace_bytes, q6w_stream_t stream) {
@@ -282,6 +287,7 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
     return fail(Q6W_ERR_ARG, "%s: the workspace needs %zu bytes", who, need);
   if (!aligned(workspace, 256)) return fail(Q6W_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
   cudaStream_t s = (cudaStream_t)stream;
+  const int64_t stall = g_stall_cycles.load(std::memory_order_relaxed);
   const float scale = (float)(1.4426950408889634 / sqrt((double)hd));
   if (b.starts && zero_padding) {
     st = zero_padding_rows(b, output, n_heads * hd, s);
@@ -323,6 +329,8 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
     d.hd = hd;
     d.scale = scale;
     d.desc = reinterpret_cast<int4*>(r.decode);
+    d.stall = stall != 0;
+    d.wait_cycles = stall ? stall : (int64_t)kWaitCycles;
     st = decode_attention(d, half, s);
   }
   if (st || prefix_length == 0) return st;
@@ -414,4 +422,12 @@ extern "C" int32_t q6w_shared_prefix_attention(const q6w_paged_batch* batch, con
                                                q6w_stream_t stream) {
   return paged::attention("q6w_shared_prefix_attention", batch, prefix_pages, prefix_length, n_tokens, n_heads, queries,
                           query_stride, output, zero_padding, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t q6w_selftest_paged_stall(int64_t wait_cycles) {
+  clear_error();
+  if (wait_cycles < 0 || wait_cycles > (int64_t(1) << 31))
+    return fail(Q6W_ERR_ARG, "q6w_selftest_paged_stall: wait_cycles must be in [0, 2^31]");
+  paged::g_stall_cycles.store(wait_cycles, std::memory_order_relaxed);
+  return Q6W_OK;
 }

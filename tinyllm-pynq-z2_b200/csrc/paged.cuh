@@ -103,6 +103,8 @@ struct DecodeArgs {
   int32_t hd, F;       // head_dim, kv heads side by side
   int32_t swap;        // the pool's map holds slots in front of kv heads
   float scale;         // log2(e) / sqrt(head_dim)
+  int32_t stall;       // the first CTA's first tiles never arrive (q6w_selftest_paged_stall)
+  int64_t wait_cycles; // bound of a wait
 };
 
 // One query token a sequence; workspace (desc): decode_workspace bytes.

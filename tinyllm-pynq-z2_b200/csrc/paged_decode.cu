@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
   }
-  if (lane < STG) mbar_init(bar + lane, 1);
+  if (lane < STG) mbar_init(bar + lane, a.stall && blockIdx.x == 0 && lane == 0 ? 2 : 1);
   fence_mbar_init();
   build_line<S::KU>(b, line);
   const int KVB = b.kv_heads / a.F * a.HB;
@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     int pblk = 0;
     int pt = 0, pbase = 0, plast = -1, ids = -1;  // page ids: lane i holds the id of page pbase + i
     int istage = 0;
-    uint32_t bad = 0;  // bits 2 stage + tile: the tile has a page id out of range
+    uint32_t bad = 0;    // bits 2 stage + tile: the tile has a page id out of range
+    uint32_t armed = 0;  // bit stage: copies were started into it
     auto enter = [&]() {  // the first piece from p on that has keys
       while (p.x < p.x1 && p.key0 >= p.key1) p.next(b, KVB);
       if (p.x >= p.x1) return;
@@ -417,6 +418,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
             if (lane == 0) flag(b.status, kErrInput);
           }
         }
+        armed |= 1u << istage;
         if (lane == 0) mbar_expect_tx(bar + istage, __popc(good) * box_bytes);
         __syncwarp();
         if (ok) {
@@ -431,6 +433,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
             enter();
           }
         }
+      } else {
+        armed &= ~(1u << istage);
       }
       istage = istage + 1 == STG ? 0 : istage + 1;
     };
@@ -439,14 +443,18 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
     for (int i = 0; i < STG - 1; ++i) issue(i & 1);
     int stage = 0;
     uint32_t phase = 0;
-    bool late = false;  // a wait ran out: the warp's outputs become NaN
+    // A wait ran out: nothing more is waited for or started, and the outputs of
+    // the rest of the warp's stretch become NaN.
+    bool late = false;
     // Wait for the oldest half unit, and start the load that takes the place of
     // the one before it (which every lane has read), STG - 1 halves ahead.
     auto advance = [&](bool values) {
-      if (!mbar_try_wait(bar + stage, phase) && !mbar_wait(bar + stage, phase)) late = true;
+      if (!mbar_try_wait(bar + stage, phase) && !mbar_wait_for(bar + stage, phase, a.wait_cycles)) late = true;
+      late = __any_sync(kAll, late);
       __syncwarp();
-      issue(values != ((STG - 1) % 2 != 0));
       const uint8_t* at = ring_g + stage * S::HALF;
+      if (late) return at;
+      issue(values != ((STG - 1) % 2 != 0));
       if (++stage == STG) {
         stage = 0;
         phase ^= 1;
@@ -509,12 +517,13 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       // heads 2 c and 2 c + 1: reference (0 until a score was seen), how far a
       // score may pass it, sum of weights
       float ref0 = 0.f, ref1 = 0.f, lim0 = -INFINITY, lim1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-      for (int t0 = key0; t0 < key1; t0 += S::KU) {
+      for (int t0 = key0; t0 < key1 && !late; t0 += S::KU) {
         // ---- S^T = K q^T: key g heads 2 c, 2 c + 1, then key g + 8
         float x[NT][4];
         {
           const uint32_t nans = bad >> (2 * stage);
           const uint8_t* kr = advance(false);
+          if (late) break;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             float s0[4], s1[4], s2[4];
@@ -619,6 +628,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
         // ---- O^T += V^T P^T; M row g of tile i is the lane's dim 2 i, row g + 8 its dim 2 i + 1
         {
           const uint8_t* vr = advance(true);
+          if (late) break;
           const bool tail = t0 + S::KU > key1;  // slots behind the last key may hold anything
 #pragma unroll
           for (int j = 0; j < NVC; ++j) {
@@ -707,9 +717,17 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       if (lane == 0 && !whole) segs[2 * warp + which] = {cur.first, s, cur.block, 1, begin, end};
       cur.next(b, KVB);
     }
-    if (late) {  // the copies that are still on their way land before the CTA ends
+    if (late) {
       if (lane == 0) flag(b.status, kErrTimeout);
-      for (int i = 0; i < STG; ++i) mbar_wait(bar + i, phase);
+      // the copies that are still on their way, from the stage that was waited for
+      // on, land before the CTA ends (or one more wait runs out)
+      for (uint64_t left = a.wait_cycles; stage != istage;) {
+        if ((armed >> stage & 1) && !mbar_wait_for(bar + stage, phase, left)) left = 0;
+        if (++stage == STG) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
     }
   }
   grid_dep_launch();

@@ -30,6 +30,7 @@ EXPORTS = (
     "q6w_prefill", "q6w_quantize_rows", "q6w_linear_workspace_bytes", "q6w_linear_ex", "q6w_generate",
     "q6w_sample", "q6w_model_set_kv_dtype", "q6w_forward_all", "q6w_selftest_wait_timeout",
     "q6w_paged_append", "q6w_paged_workspace_bytes", "q6w_paged_attention", "q6w_shared_prefix_attention",
+    "q6w_selftest_paged_stall",
 )
 
 
@@ -125,6 +126,7 @@ def _declare(lib):
                                           c_void_p, c_size_t, S]),
         "q6w_shared_prefix_attention": (c_int32, [c_char_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
                                                   c_int64, c_void_p, c_int32, c_void_p, c_size_t, S]),
+        "q6w_selftest_paged_stall": (c_int32, [c_int64]),
         "q6w_gqa_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int64, S]),
     }
