@@ -466,11 +466,11 @@ Q6W_API int32_t q6w_workspace_status(void* workspace, q6w_stream_t stream);
  * status instead of a hang. */
 Q6W_API int32_t q6w_selftest_wait_timeout(void* workspace, int64_t wait_cycles, q6w_stream_t stream);
 
-/* Diagnostic of q6w_paged_attention for single tokens, with no counterpart in
- * the reference: with wait_cycles in 1 .. 2^31, later calls of this process (on
+/* Diagnostic of the paged attention calls, with no counterpart in the
+ * reference: with wait_cycles in 1 .. 2^31, later calls of this process (on
  * every thread and stream) run with waits bounded by wait_cycles SM clock
- * cycles and with tiles of cached keys that their first thread block waits for
- * in vain.  Such a call ends after a few bounds; the rows that the
+ * cycles and with tiles of cached keys that the first thread block of each
+ * kernel waits for in vain.  Such a call ends after a few bounds; the rows that the
  * block takes part in come out NaN, the others as ever, and bit 2 of the
  * batch's status is set.  0 ends the diagnostic. */
 Q6W_API int32_t q6w_selftest_paged_stall(int64_t wait_cycles);

@@ -62,3 +62,34 @@ def test_decode_wait_runs_out_in_a_piece(kv):
     """One long request: the first block's piece spoils the heads of the first kv head alone."""
     c = make(1, 16, 4, 64, 16, kv, [9000], [1], seed=5)
     assert check_stalled(c, [(0, h) for h in range(4)]) == 0.25
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("H,KV,hd", [(8, 4, 16), (16, 4, 64), (8, 4, 128)])
+def test_chunk_wait_runs_out(H, KV, hd, kv):
+    """Short chunks: the first block holds several, and the later ones of its stretch become NaN too."""
+    n = 700
+    c = make(n, H, KV, hd, 16, kv, [(i * 29) % 90 for i in range(n)], [7] * n, seed=3)
+    units = 64 if kv == torch.float32 else 128
+    stretch = sum(max(1, -(-int(x) // units)) for x in c["lens"]) * KV // 148  # units of the first block
+    share = check_stalled(c, [(t, h) for t in range(7 * (stretch // (2 * KV))) for h in range(H)])
+    assert share < 0.02
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd,tokens", [(64, 64), (128, 32)])
+def test_chunk_wait_runs_out_in_a_piece(hd, tokens, kv):
+    """One long chunk: the first block's piece spoils its 256 (128) rows alone."""
+    c = make(1, 8, 2, hd, 16, kv, [3000], [300], seed=6)
+    share = check_stalled(c, [(t, h) for t in range(tokens) for h in range(4)])
+    assert share == pytest.approx(tokens * 4 / (300 * 8))
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("new", [1, 5])
+def test_prefix_wait_runs_out(new, kv):
+    """The prefix's first block holds a piece of the first kv head's rows; the sequences' own first block others."""
+    n = 60 // new
+    c = make(n, 8, 2, 64, 16, kv, [40 * i for i in range(n)], [new] * n, seed=7, prefix=3000)
+    share = check_stalled(c, [(t, h) for t in range(n * new) for h in range(4)])
+    assert share < 0.75

@@ -305,6 +305,8 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
   t.H = n_heads;
   t.scale = scale;
   t.prefix_len = prefix_length;
+  t.stall = stall != 0;
+  t.wait_cycles = stall ? stall : (int64_t)kWaitCycles;
   TcArgs pre = t;
   pre.part = r.prefix;
   pre.part_ml = r.prefix_ml;
@@ -329,8 +331,8 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
     d.hd = hd;
     d.scale = scale;
     d.desc = reinterpret_cast<int4*>(r.decode);
-    d.stall = stall != 0;
-    d.wait_cycles = stall ? stall : (int64_t)kWaitCycles;
+    d.stall = t.stall;
+    d.wait_cycles = t.wait_cycles;
     st = decode_attention(d, half, s);
   }
   if (st || prefix_length == 0) return st;

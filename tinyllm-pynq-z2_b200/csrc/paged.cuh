@@ -127,6 +127,8 @@ struct TcArgs {
   int32_t H, swap;
   int32_t prefix, prefix_len, items;  // over the prefix (its pages in b.table), blocks of all kv heads
   float scale;       // log2(e) / sqrt(head_dim)
+  int32_t stall;     // as DecodeArgs
+  int64_t wait_cycles;
 };
 
 struct TcMaps {

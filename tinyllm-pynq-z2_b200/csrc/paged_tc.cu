@@ -40,7 +40,7 @@
 //
 // Blocks' units lie on one line; every CTA takes an equal stretch (as the
 // decode kernel's warps do).  Every wait is bounded; a timeout sets the status
-// bit and makes the CTA stop.
+// bit, makes the CTA stop and its rows NaN.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   if (tid == 0) {
     if (!a.prefix) a.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
     for (int i = 0; i < STG; ++i) {
-      mbar_init(k_full + i, 4);
+      mbar_init(k_full + i, a.stall && blockIdx.x == 0 && i == 0 ? 5 : 4);
       mbar_init(v_full + i, 4);
       mbar_init(k_empty + i, 1);
       mbar_init(v_empty + i, 1);
@@ -421,12 +421,13 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   const int64_t x0 = w.p.x;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (stop) return false;
-    if (mbar_try_wait(bar, parity) || mbar_wait(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity) || mbar_wait_for(bar, parity, a.wait_cycles)) return true;
     stop = 1;
     flag(a.b.status, kErrTimeout);
     return false;
   };
   auto tile_col = [&](int t) { return tmem + t * S::TC; };
+  int loaded = 0;  // units that this (load) warp put into shared memory
 
   if (warp >= S::SOFT && warp < S::SOFT + 4) {
     // ---- loads
@@ -602,13 +603,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         }
       }
     }
-    if (kHalf && lw == 0 && stop) {
-      // copies that are still on their way land before the CTA ends
-      for (int st = 0; st < STG && st < i; ++st) {
-        mbar_wait(k_full + st, ((i - 1 - st) / STG) & 1);
-        mbar_wait(v_full + st, ((i - 1 - st) / STG) & 1);
-      }
-    }
+    loaded = i;
   } else if (warp >= S::SOFT + 4) {
     // ---- MMAs
     set_registers<S::REGS, S::MMA_REGS>();
@@ -756,8 +751,8 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       return mine;
     };
     uint32_t sn = 0, s_seen[2] = {0, 0}, done = 0;
-    bool ok = true;
-    for (; ok && w.more(); w.next()) {
+    bool ok = true;  // false: a wait ran out, and the rows of this and all later pieces become NaN
+    for (; w.more(); w.next()) {
       if (TILES == 2 && t == 1 && w.rows() <= 128) continue;
       const int ri = w.p.j * S::ROWS + t * 128 + r;  // row of the (sequence, kv head)
       const bool in = t * 128 + r < w.rows();
@@ -765,7 +760,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       const int64_t token = w.p.tok0 + tok;
       const int vis = in ? w.seen(tok) : 0;
       float sc = a.scale;
-      {
+      if (ok) {
         // Q's parts into tensor memory, two elements a column
         const float* qp = a.q + token * a.ldq + (int64_t)h * HD;
         float down = 1.f;
@@ -813,7 +808,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
 #pragma unroll
       for (int d = 0; d < MYD; ++d) acc[d] = 0.f;
       float ref = 0.f, lim = -INFINITY, l = 0.f;
-      for (int u = w.p.u0; u < w.p.u1; ++u) {
+      for (int u = ok ? w.p.u0 : w.p.u1; u < w.p.u1; ++u) {
         const int buf = TILES == 2 ? t : (int)(sn & 1);
         ok = wait(s_full + buf, s_seen[buf]++ & 1) && ok;
         if (HALVES == 1) {
@@ -927,7 +922,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       ok = agree(ok);
       if constexpr (HALVES == 2) l += row_sum[hf ^ 1][r];
       if (!ok) {
-        l = NAN;  // a wait ran out: the rows become NaN
+        l = NAN;
       } else {
         tc::tc_fence_after();
 #pragma unroll
@@ -978,6 +973,15 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     }
   }
   __syncthreads();
+  if (kHalf && warp == S::SOFT && stop) {
+    // copies that are still on their way land before the CTA ends (or one more wait runs out)
+    uint64_t left = a.wait_cycles;
+    for (int st = 0; st < STG && st < loaded; ++st) {
+      const uint32_t par = ((loaded - 1 - st) / STG) & 1;
+      if (!mbar_wait_for(k_full + st, par, left)) left = 0;
+      if (!mbar_wait_for(v_full + st, par, left)) left = 0;
+    }
+  }
   if (warp == S::SOFT + 4) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
