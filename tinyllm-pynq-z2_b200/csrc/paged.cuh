@@ -81,6 +81,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The FP16 parts of a row x of queries (FP16 pages) are those of x 2^e with the
+// largest element in [2^14, 2^15): elements down to 2^-17 of it keep 22 bits, as
+// their low parts are then normal FP16 numbers; smaller ones err by 2^-39 of the
+// largest.  Returns 2^e; back becomes 2^-e.
+__device__ __forceinline__ float half_scale(float largest, float& back) {
+  const int ex = min(max((int)(__float_as_uint(largest) >> 23), 15), 254);
+  back = __uint_as_float((uint32_t)(ex - 14) << 23);
+  return __uint_as_float((uint32_t)(268 - ex) << 23);
+}
 // A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 

@@ -17,8 +17,8 @@
 // and a lane can load its part of K and V straight from the cache.
 //
 // Precision.  FP16 keys and values are exact operands; queries (scaled by a
-// power of two per head) and weights enter as two FP16 parts, hi + lo, 22
-// bits.  FP32 keys, values, queries and weights enter as two TF32 parts and
+// power of two per head, half_scale) and weights enter as two FP16 parts, hi + lo,
+// 22 bits.  FP32 keys, values, queries and weights enter as two TF32 parts and
 // the products hi hi + hi lo + lo hi, dropping terms of 2^-22.  The MMA adds
 // in FP32; a tile's output is added to o in registers, rounded to nearest, so
 // no long sum lives in the MMA's accumulator.
@@ -498,14 +498,12 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           for (int i = 0; i < HDF / 4; ++i) mx = fmaxf(mx, fabsf(qv[i]));
           mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
-          // 2^-e with 2^e the power of two at or below the head's largest element
-          const int ex = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
-          const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = __uint_as_float((uint32_t)ex << 23);
-          const float us = a.scale * up;
+          float back;
+          const float scale = half_scale(mx, back), us = a.scale * back;
           sc0 = __shfl_sync(kAll, us, 8 * c);
           sc1 = __shfl_sync(kAll, us, 8 * c + 4);
 #pragma unroll
-          for (int i = 0; i < 2 * QS; ++i) split_f16(qv[2 * i] * down, qv[2 * i + 1] * down, qhi[i], qlo[i]);
+          for (int i = 0; i < 2 * QS; ++i) split_f16(qv[2 * i] * scale, qv[2 * i + 1] * scale, qhi[i], qlo[i]);
         } else {
 #pragma unroll
           for (int i = 0; i < 2 * QS; ++i) split_tf32(__float_as_uint(qv[i]), qhi[i], qlo[i]);

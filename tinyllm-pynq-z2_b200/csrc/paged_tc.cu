@@ -9,7 +9,7 @@
 // block's keys join as in the decode kernel.
 //
 // Operands.  FP16 pages: K and V enter as they are, Q (scaled by a power of
-// two a row) and P as FP16 hi + lo, 22 bits: 2 + 2 MMAs.  FP32 pages: every
+// two a row, half_scale) and P as FP16 hi + lo, 22 bits: 2 + 2 MMAs.  FP32 pages: every
 // operand enters as three BF16 parts (24 bits) and the products down to
 // 2^-16 are kept, 6 + 6 MMAs, the small ones first.  Q and P are the MMA's A
 // operand and live in tensor memory, where the softmax threads (one row each:
@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       if (ok) {
         // Q's parts into tensor memory, two elements a column
         const float* qp = a.q + token * a.ldq + (int64_t)h * HD;
-        float down = 1.f;
+        float scale = 1.f;
         if (kHalf) {
           float mx = 0.f;
           if (in)
@@ -771,9 +771,9 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
               const float4 v = __ldg(reinterpret_cast<const float4*>(qp + e));
               mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
             }
-          const int ex = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
-          down = __uint_as_float((uint32_t)(254 - ex) << 23);
-          sc *= __uint_as_float((uint32_t)ex << 23);
+          float back;
+          scale = half_scale(mx, back);
+          sc *= back;
         }
 #pragma unroll 2
         for (int e0 = hf * MYD; e0 < (hf + 1) * MYD; e0 += 16) {
@@ -783,8 +783,8 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (in) v = __ldg(reinterpret_cast<const float4*>(qp + e0 + e));
             uint32_t x[QP], y[QP];
-            split_pair<kHalf, QP>(v.x * down, v.y * down, x);
-            split_pair<kHalf, QP>(v.z * down, v.w * down, y);
+            split_pair<kHalf, QP>(v.x * scale, v.y * scale, x);
+            split_pair<kHalf, QP>(v.z * scale, v.w * scale, y);
 #pragma unroll
             for (int q = 0; q < QP; ++q) {
               part[q][e / 2] = x[q];
