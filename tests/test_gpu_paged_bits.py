@@ -13,26 +13,28 @@ pytestmark = pytest.mark.gpu
 
 
 def fill(c, keys, values):
-    """keys / values [N, hd] (the same in every sequence and kv head) into the pages."""
-    ps = c["kp"].shape[1]
+    """keys / values [N, hd], those of a shared prefix first, into the pages of every sequence and kv head."""
+    ps, P = c["kp"].shape[1], c["prefix"]
     c["kp"].zero_()
     c["vp"].zero_()
-    for i, (a, b) in enumerate(zip(c["past"], c["new"])):
-        at = torch.arange(a + b, device="cuda")
-        page = c["table"][i][at // ps].long()
-        c["kp"][page, at % ps] = keys[: a + b, None].to(c["kp"].dtype)
-        c["vp"][page, at % ps] = values[: a + b, None].to(c["vp"].dtype)
+    parts = [(c["prefix_pages"], 0, P)] + [(row, P, a + b) for row, a, b in zip(c["table"], c["past"], c["new"])]
+    for pages, first, count in parts:
+        at = torch.arange(count, device="cuda")
+        for pool, x in ((c["kp"], keys), (c["vp"], values)):
+            pool[pages[at // ps].long(), at % ps] = x[first: first + count, None].to(pool.dtype)
 
 
 def softmax64(c, scores, values):
     """Rows [T, H, hd] for scores [H, N] that do not depend on the token, and the weights behind them."""
-    out, weights = [], []
+    made, order = {}, []
     for a, b in zip(c["past"], c["new"]):
         for j in range(b):
-            w = torch.softmax(scores[:, : a + j + 1].double(), -1)
-            out.append(w @ values[: a + j + 1].double())
-            weights.append(w)
-    return torch.stack(out), weights
+            seen = c["prefix"] + a + j + 1
+            if seen not in made:
+                w = torch.softmax(scores[:, :seen].double(), -1)
+                made[seen] = (w @ values[:seen].double(), w)
+            order.append(seen)
+    return torch.stack([made[s][0] for s in order]), [made[s][1] for s in order]
 
 
 @pytest.mark.parametrize("outlier,kv", [(x, torch.float32) for x in (0.0, 1e3, -1e5, 1e20)] +
@@ -68,3 +70,38 @@ def test_a_large_query_element_does_not_cost_the_others_their_bits(outlier, new,
     err = ((got - want).abs() / want.clamp(min=1e-300)).masked_fill(want == 0, 0.0)
     assert not got[want == 0].any()
     assert float(err.max()) <= 2 * delta + (4 + N + 8) * U
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("n,past,new,prefix", [(2, 4090, 1, 0), (1500, 200, 1, 0), (2, 4090, 5, 0), (2, 30, 1, 4000),
+                                               (2, 30, 5, 4000)])
+@pytest.mark.parametrize("above", [0, 6, 14, 17, 20, 22])
+def test_many_small_weights_behind_a_sink(above, n, past, new, prefix, hd, kv):
+    """The first key's weight is some 2^``above`` times those of the others, which are
+    equal, and its value is 0: the output is what the small weights make of theirs.
+    Relative to W = sum w |v|: 2 delta (as above); sums that a tensor core cuts, of up
+    to 512 products before registers add them, 2 u each, and pieces of them, 1200 u;
+    the sum of weights and the quotient, 300 u.  FP16 pages: a weight errs by 2^-37 of
+    the largest."""
+    H, N = 8, prefix + past + new
+    c = make(n, H, 2, hd, 16, kv, [past] * n, [new] * n, seed=hd, prefix=prefix)
+    g = torch.Generator().manual_seed(above)
+    keys = torch.zeros(N, hd)
+    keys[:, 1] = -0.3
+    keys[0, 1] = above * math.log(2.0)
+    keys = keys.half().float()
+    values = torch.rand(N, hd, generator=g).half().float()
+    values[0] = 0
+    fill(c, keys.cuda(), values.cuda())
+    c["q"].zero_()
+    x = math.sqrt(hd) * torch.linspace(0.9, 1.0, H)
+    c["q"][..., 1] = x.cuda()
+    got = attend(c).double().cpu()
+    scores = x.double()[:, None] * keys[None, :, 1].double() / math.sqrt(hd)
+    want, weights = softmax64(c, scores, values)
+    W = torch.stack([w @ values[: w.shape[1]].abs().double() for w in weights])
+    tol = (2 * 12 * U * float(scores.abs().max()) + 1500 * U) * W
+    if kv == torch.float16:
+        tol += torch.stack([2.0 ** -37 * w.amax(-1, keepdim=True) * values[: w.shape[1]].abs().double().sum(0) for w in weights])
+    assert float(((got - want).abs() / tol).max()) <= 1.0

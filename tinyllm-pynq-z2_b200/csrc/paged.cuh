@@ -90,6 +90,18 @@ __device__ __forceinline__ float half_scale(float largest, float& back) {
   back = __uint_as_float((uint32_t)(ex - 14) << 23);
   return __uint_as_float((uint32_t)(268 - ex) << 23);
 }
+// Weights are 2^(s - m), m a reference that starts kFirst below the first maximum
+// and moves when a score passes it by more than kLimit, so that the largest weight
+// lies in [2^kFirst, 2^kLimit].  FP16 parts: close under FP16's largest number
+// (65504 > 2^15.9), so that weights down to 2^-(kFirst + 3) of the largest keep 22
+// bits (their low parts are normal numbers) and smaller ones err by 2^-(kFirst + 25)
+// of it at most -- many small weights may outweigh a sink whose value is 0.  FIRST
+// nearer to kLimit moves the reference more often.  FP32's range needs no such care.
+template <bool HALF, int FIRST>
+struct Weights {
+  static constexpr float kFirst = HALF ? FIRST : 0;
+  static constexpr float kLimit = HALF ? 15.9f : 8.f;
+};
 // A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 

@@ -2,7 +2,7 @@
 //
 // Mathematics.  One pass over the keys with a reference exponent m, a sum l and
 // an output o per query head: p = 2^(s - m), l += p, o += p v; m follows the
-// largest score so far (it moves only when a score passes it by more than 8,
+// largest score so far (it moves only when a score passes it by a bound, Weights;
 // then l and o are scaled by 2^(m_old - m_new)).  States of disjoint key
 // ranges join as m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m).
 //
@@ -330,7 +330,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   constexpr int NT = S::NT;                  // tiles of a unit
   constexpr int MT = HDF / 16;               // M tiles of O^T
   constexpr int QS = kHalf ? HDF / 16 : HDF / 8;  // K steps of S
-  constexpr float kOff = kHalf ? 4.f : 0.f;  // FP16 weights reach 2^(kOff + 8): their low parts stay normal
+  using Wt = Weights<kHalf, 14>;  // (moving the reference is a few instructions here)
+  constexpr float kFirst = Wt::kFirst, kLimit = Wt::kLimit;
   constexpr unsigned kAll = 0xffffffffu;
   extern __shared__ uint8_t smem_raw[];  // [warp][RING], 1024-byte aligned
   __shared__ uint64_t bars[kDecodeWarps * STG];
@@ -577,11 +578,11 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           }
           // (a head that has seen nothing has l = o = 0: any factor will do)
           const bool seen0 = lim0 != -INFINITY, seen1 = lim1 != -INFINITY;
-          const float n0 = seen0 ? fmaxf(m0 - kOff, ref0) : (m0 == -INFINITY ? 0.f : m0 - kOff);
-          const float n1 = seen1 ? fmaxf(m1 - kOff, ref1) : (m1 == -INFINITY ? 0.f : m1 - kOff);
+          const float n0 = seen0 ? fmaxf(m0 - kFirst, ref0) : (m0 == -INFINITY ? 0.f : m0 - kFirst);
+          const float n1 = seen1 ? fmaxf(m1 - kFirst, ref1) : (m1 == -INFINITY ? 0.f : m1 - kFirst);
           const float f0 = seen0 ? ex2(ref0 - n0) : 1.f, f1 = seen1 ? ex2(ref1 - n1) : 1.f;
-          if (m0 != -INFINITY) lim0 = kOff + 8.f;
-          if (m1 != -INFINITY) lim1 = kOff + 8.f;
+          if (m0 != -INFINITY) lim0 = kLimit;
+          if (m1 != -INFINITY) lim1 = kLimit;
           ref0 = n0;
           ref1 = n1;
           l0 *= f0;

@@ -5,7 +5,7 @@
 // the `rep` heads of the group: row = token rep + r.  A CTA holds a block of
 // 128 (256) rows and walks over its keys in units of 128 (FP16 pages) or 64
 // (FP32): S = Q K^T, p = 2^(c s - m) with a reference m a row that moves only
-// when a score passes it by more than 8, l += p, O += P V.  Pieces of a
+// when a score passes it by a bound (Weights), l += p, O += P V.  Pieces of a
 // block's keys join as in the decode kernel.
 //
 // Operands.  FP16 pages: K and V enter as they are, Q (scaled by a power of
@@ -729,7 +729,11 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     const int t = TILES == 2 ? warp >> 2 : 0, hf = HALVES == 2 ? warp >> 2 : 0, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t qcol = tile_col(t) + lanes, scol = qcol + S::QC, ocol = scol + BUFS * S::SC + hf * (HD / HALVES);
-    constexpr float kOff = kHalf ? 4.f : 0.f;  // FP16 weights reach 2^(kOff + 8): their low parts stay normal
+    // Moving the reference waits for the last PV and rewrites O: 2 x 2048 tokens behind up
+    // to 6144, some heads sharp, take 870 us with 14, 836 with 12 (825 with 4, where a weight 2^-14 of the largest
+    // keeps 15 bits).
+    using Wt = Weights<kHalf, 12>;
+    constexpr float kFirst = Wt::kFirst, kLimit = Wt::kLimit;
     constexpr int NCH = KEYS / 32 / HALVES;    // 32-key chunks of a unit that this thread takes
     constexpr int MYD = HD / HALVES;           // dims of O that this thread takes
     const int ch0 = hf * NCH;
@@ -866,9 +870,9 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         }
         if (grow) {
           const bool seen = lim != -INFINITY;
-          const float m = seen ? fmaxf(mx - kOff, ref) : (mx == -INFINITY ? 0.f : mx - kOff);
+          const float m = seen ? fmaxf(mx - kFirst, ref) : (mx == -INFINITY ? 0.f : mx - kFirst);
           const float f = seen ? ex2(ref - m) : 1.f;
-          if (mx != -INFINITY) lim = kOff + 8.f;
+          if (mx != -INFINITY) lim = kLimit;
           ref = m;
           l *= f;
           if (uu > 0 && !flush) {
