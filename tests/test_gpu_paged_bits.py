@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import U, attend, make
+from test_gpu_paged import U, attend, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,14 @@ def test_many_small_weights_behind_a_sink(above, n, past, new, prefix, hd, kv):
     if kv == torch.float16:
         tol += torch.stack([2.0 ** -37 * w.amax(-1, keepdim=True) * values[: w.shape[1]].abs().double().sum(0) for w in weights])
     assert float(((got - want).abs() / tol).max()) <= 1.0
+
+
+@pytest.mark.parametrize("new,prefix", [(1, 0), (40, 0), (1, 200), (40, 200)])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+def test_large_float32_values_do_not_overflow(hd, new, prefix):
+    """Values close to FP32's largest: every output is a mean of them, so it is finite."""
+    c = make(3, 8, 2, hd, 16, torch.float32, [70, 3, 200], [new] * 3, seed=hd, prefix=prefix)
+    c["vp"].clamp_(-1, 1).mul_(3.3e38)
+    out = attend(c)
+    assert bool(out.isfinite().all())
+    check(c, out)

@@ -9,6 +9,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "async.cuh"
 #include "common.cuh"
@@ -96,12 +97,16 @@ __device__ __forceinline__ float half_scale(float largest, float& back) {
 // (65504 > 2^15.9), so that weights down to 2^-(kFirst + 3) of the largest keep 22
 // bits (their low parts are normal numbers) and smaller ones err by 2^-(kFirst + 25)
 // of it at most -- many small weights may outweigh a sink whose value is 0.  FIRST
-// nearer to kLimit moves the reference more often.  FP32's range needs no such care.
+// nearer to kLimit moves the reference more often.  FP32 pages: weights of at most 1,
+// so that values up to FP32's largest do not overflow where their mean does not.
 template <bool HALF, int FIRST>
 struct Weights {
-  static constexpr float kFirst = HALF ? FIRST : 0;
-  static constexpr float kLimit = HALF ? 15.9f : 8.f;
+  static constexpr float kFirst = HALF ? FIRST : -8;
+  static constexpr float kLimit = HALF ? 15.9f : 0.f;
 };
+// A row's reference while it has seen no score.  (Weights behind it are 0: their
+// scores are -inf.)
+constexpr float kUnseen = -FLT_MAX;
 // A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 

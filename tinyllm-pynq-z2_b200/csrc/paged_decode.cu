@@ -513,9 +513,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       float acc[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-      // heads 2 c and 2 c + 1: reference (0 until a score was seen), how far a
-      // score may pass it, sum of weights
-      float ref0 = 0.f, ref1 = 0.f, lim0 = -INFINITY, lim1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      // heads 2 c and 2 c + 1: reference, sum of weights
+      float ref0 = kUnseen, ref1 = kUnseen, l0 = 0.f, l1 = 0.f;
       for (int t0 = key0; t0 < key1 && !late; t0 += S::KU) {
         // ---- S^T = K q^T: key g heads 2 c, 2 c + 1, then key g + 8
         float x[NT][4];
@@ -570,19 +569,15 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
         }
         m0 *= sc0;
         m1 *= sc1;
-        if (__any_sync(kAll, m0 - ref0 > lim0 || m1 - ref1 > lim1)) {
+        if (__any_sync(kAll, m0 - ref0 > kLimit || m1 - ref1 > kLimit)) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(kAll, m0, o));
             m1 = fmaxf(m1, __shfl_xor_sync(kAll, m1, o));
           }
-          // (a head that has seen nothing has l = o = 0: any factor will do)
-          const bool seen0 = lim0 != -INFINITY, seen1 = lim1 != -INFINITY;
-          const float n0 = seen0 ? fmaxf(m0 - kFirst, ref0) : (m0 == -INFINITY ? 0.f : m0 - kFirst);
-          const float n1 = seen1 ? fmaxf(m1 - kFirst, ref1) : (m1 == -INFINITY ? 0.f : m1 - kFirst);
-          const float f0 = seen0 ? ex2(ref0 - n0) : 1.f, f1 = seen1 ? ex2(ref1 - n1) : 1.f;
-          if (m0 != -INFINITY) lim0 = kLimit;
-          if (m1 != -INFINITY) lim1 = kLimit;
+          // (a head that has seen nothing has l = o = 0: the factor 0 keeps them)
+          const float n0 = fmaxf(m0 - kFirst, ref0), n1 = fmaxf(m1 - kFirst, ref1);
+          const float f0 = ex2(ref0 - n0), f1 = ex2(ref1 - n1);
           ref0 = n0;
           ref1 = n1;
           l0 *= f0;
@@ -704,7 +699,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           }
         }
         if ((!whole || a.state) && g == 0) {
-          const float m = (hh ? lim1 : lim0) == -INFINITY ? -INFINITY : (hh ? ref1 : ref0);
+          const float ref = hh ? ref1 : ref0, m = ref == kUnseen ? -INFINITY : ref;
           if (!whole) {
             slot[8 * a.hd + n] = m;
             slot[8 * a.hd + 8 + n] = l;

@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       float acc[MYD];
 #pragma unroll
       for (int d = 0; d < MYD; ++d) acc[d] = 0.f;
-      float ref = 0.f, lim = -INFINITY, l = 0.f;
+      float ref = kUnseen, l = 0.f;
       for (int u = ok ? w.p.u0 : w.p.u1; u < w.p.u1; ++u) {
         const int buf = TILES == 2 ? t : (int)(sn & 1);
         ok = wait(s_full + buf, s_seen[buf]++ & 1) && ok;
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         mx *= sc;
         const int uu = u - w.p.u0;
         const bool flush = uu > 0 && uu % S::kFlush == 0;
-        const bool grow = __any_sync(0xffffffffu, mx - ref > lim);
+        const bool grow = __any_sync(0xffffffffu, mx - ref > kLimit);
         // Every PV is waited for, in order and before the weights that let the next
         // one start are handed over: a parity tells a phase from its neighbours only.
         // Here when O is needed, else behind the arithmetic.
@@ -869,10 +869,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           }
         }
         if (grow) {
-          const bool seen = lim != -INFINITY;
-          const float m = seen ? fmaxf(mx - kFirst, ref) : (mx == -INFINITY ? 0.f : mx - kFirst);
-          const float f = seen ? ex2(ref - m) : 1.f;
-          if (mx != -INFINITY) lim = kLimit;
+          const float m = fmaxf(mx - kFirst, ref), f = ex2(ref - m);
           ref = m;
           l *= f;
           if (uu > 0 && !flush) {
@@ -940,7 +937,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       }
       if (in) {
         const bool begin = w.p.u0 == 0, whole = begin && w.p.u1 == w.p.units;
-        const float m = lim == -INFINITY ? -INFINITY : ref;
+        const float m = ref == kUnseen ? -INFINITY : ref;
         float* dst;
         float* ml;
         float inv = 1.f;
