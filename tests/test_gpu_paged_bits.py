@@ -116,3 +116,21 @@ def test_large_float32_values_do_not_overflow(hd, new, prefix):
     out = attend(c)
     assert bool(out.isfinite().all())
     check(c, out)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("value", [torch.finfo(torch.float32).min, 3.395e38, math.inf])
+def test_a_later_value_of_any_size_stays_in_its_rows(value, hd):
+    """Chunks over FP32 pages: rows that do not see a key do not meet its value, FP32's lowest among them."""
+    c = make(2, 8, 2, hd, 16, torch.float32, [30, 0], [50, 20], seed=hd)
+    want = attend(c)
+    c["vp"][int(c["table"][0, 65 // 16]), 65 % 16] = value
+    got = attend(c)
+    assert torch.equal(got[:35], want[:35]) and torch.equal(got[50:], want[50:])
+    if value == math.inf:
+        assert not got[35:50].isfinite().any()
+    else:
+        c["q"] /= 64  # even weights: a mean with one such value
+        got = attend(c)
+        assert bool(got.isfinite().all())
+        check(c, got)

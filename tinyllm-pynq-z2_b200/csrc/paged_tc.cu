@@ -199,7 +199,17 @@ __device__ __forceinline__ bool load_warps_agree(bool ok) {
   return r != 0;
 }
 
-// Two values -> packed parts, first value in the low half.
+// (x, y) -> BF16, rounded to nearest; what would round to infinity becomes the
+// largest number (infinity too).
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+  uint32_t w;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  return w;
+}
+
+// Two values -> packed parts, first value in the low half.  BF16: the first part of
+// a value close to FP32's largest must not round to infinity (a hidden key's weight of
+// 0 would make it NaN); of an infinity the second part is one.
 template <bool HALF_PARTS, int N>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&w)[N]) {
 #pragma unroll
@@ -214,7 +224,7 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&w)[N]) {
       }
     } else {
       const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      w[i] = i == 0 ? bf16_pair(x, y) : *reinterpret_cast<const uint32_t*>(&h);
       if (i + 1 < N) {
         x -= __uint_as_float(w[i] << 16);
         y -= __uint_as_float(w[i] & 0xffff0000u);
