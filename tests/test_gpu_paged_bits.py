@@ -134,3 +134,33 @@ def test_a_later_value_of_any_size_stays_in_its_rows(value, hd):
         got = attend(c)
         assert bool(got.isfinite().all())
         check(c, got)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("H,KV,hd,ps", [(8, 4, 16, 16), (4, 4, 16, 8), (8, 2, 32, 2), (16, 2, 64, 16), (10, 2, 128, 32)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_keys_that_are_not_finite(value, H, KV, hd, ps, kv):
+    """Single tokens: an element of one kv head's keys that is not finite is no
+    business of the other kv heads, and a score of -inf is a weight of 0."""
+    lens = [5, 17, 64, 130, 400]
+    c = make(len(lens), H, KV, hd, ps, kv, [x - 1 for x in lens], [1] * len(lens), seed=hd)
+    struck = [(i, g, at) for i, x in enumerate(lens) for g, at in ((i % KV, x // 2), ((i + 1) % KV, x - 1))]
+    for i, g, at in struck:
+        c["kp"][int(c["table"][i, at // ps]), at % ps, g, (3 * i) % hd] = value
+    got = attend(c).double()
+    for i, x in enumerate(lens):
+        page = c["table"][i, : -(-x // ps)].long()
+        k, v = (pool[page].flatten(0, 1)[:x].double() for pool in (c["kp"], c["vp"]))
+        q = c["q"][i].double().unflatten(0, (KV, H // KV))
+        s = torch.einsum("grd,kgd->grk", q, k) / math.sqrt(hd)
+        w = torch.softmax(s, -1)
+        want = torch.einsum("grk,kgd->grd", w, v).flatten(0, 1)
+        W = torch.einsum("grk,kgd->grd", w, v.abs()).flatten(0, 1)
+        A = torch.einsum("grd,kgd->grk", q.abs(), torch.where(k.isfinite(), k.abs(), 0)).amax(-1).flatten() / math.sqrt(hd)
+        tol = (2 * (hd + 16) * U * A[:, None] + (2 * x + 16) * U) * W
+        finite = want.isfinite()
+        assert torch.equal(got[i].isfinite(), finite), (i, value)
+        assert bool(((got[i] - want).abs() <= tol)[finite].all())
+    hit = {(i, g) for i, g, _ in struck}
+    clean = torch.tensor([[(i, g) not in hit for g in range(KV)] for i in range(len(lens))]).repeat_interleave(H // KV, 1)
+    assert bool(got[clean.cuda()].isfinite().all())

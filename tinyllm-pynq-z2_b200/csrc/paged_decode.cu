@@ -306,6 +306,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// The larger of two values, NaN if either is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
 // x = hi + lo as TF32 operands: hi rounded to nearest (11 bits), lo the exact
 // rest, of which the MMA takes the upper 11 bits.  A NaN stays one in lo.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
@@ -319,6 +326,18 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
   const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// q . K of one row of a tile in shared memory, one FP32 product after the other; the
+// kv head's elements start at element `first` of the row.
+template <int HDF, typename KT>
+__device__ __noinline__ float plain_score(const float* q, const uint8_t* tile, int row, int first, int hd) {
+  using S = DecodeShape<HDF, KT>;
+  float dot = 0.f;
+#pragma unroll 1
+  for (int d = 0; d < hd; ++d)
+    dot = fmaf(__ldg(q + d), (float)*reinterpret_cast<const KT*>(tile + S::place(row, (first + d) * S::ES)), dot);
+  return dot;
 }
 
 template <int HDF, typename KT>
@@ -562,14 +581,35 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           }
         }
         // ---- the references, when a score passes them by too much
-        float m0 = fmaxf(x[0][0], x[0][2]), m1 = fmaxf(x[0][1], x[0][3]);
+        float m0 = max_nan(x[0][0], x[0][2]), m1 = max_nan(x[0][1], x[0][3]);
         if constexpr (NT == 2) {
-          m0 = fmaxf(m0, fmaxf(x[1][0], x[1][2]));
-          m1 = fmaxf(m1, fmaxf(x[1][1], x[1][3]));
+          m0 = max_nan(m0, max_nan(x[1][0], x[1][2]));
+          m1 = max_nan(m1, max_nan(x[1][1], x[1][3]));
         }
         m0 *= sc0;
         m1 *= sc1;
-        if (__any_sync(kAll, m0 - ref0 > kLimit || m1 - ref1 > kLimit)) {
+        if (__any_sync(kAll, !(m0 - ref0 <= kLimit && m1 - ref1 <= kLimit))) {
+          // A score that is not a number may be another kv head's doing (its infinite
+          // key times this head's zeros), or the parts' (inf - inf): it is computed again
+          // from the tile, unless a page was missing.
+          const int st = stage == 0 ? STG - 1 : stage - 1;
+          m0 = m1 = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int n = 2 * c + (i & 1);
+              if (x[t][i] != x[t][i] && n < nr && !(bad >> (2 * st + t) & 1)) {
+                const float dot = plain_score<HDF, KT>(a.q + s * a.ldq + (int64_t)(h0 + n) * a.hd,
+                                                       ring_g + st * S::HALF + t * S::TILE, krow + 8 * (i >> 1),
+                                                       fc[i & 1] * a.hd, a.hd);
+                x[t][i] = kHalf ? dot * (a.scale / (i & 1 ? sc1 : sc0)) : dot;
+              }
+              if (i & 1) m1 = fmaxf(m1, x[t][i]); else m0 = fmaxf(m0, x[t][i]);
+            }
+          }
+          m0 *= sc0;
+          m1 *= sc1;
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(kAll, m0, o));
