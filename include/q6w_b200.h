@@ -371,8 +371,10 @@ Q6W_API int32_t q6w_sample(const float* logits, int64_t ld, int32_t n, int32_t v
  * written); a token whose position is negative (more new tokens than the
  * length) or that no sequence holds (in front of query_starts[0], behind
  * query_starts[n_seqs]) is padding; a page id outside [0, n_pages) is never
- * followed.  Such a length and a bad page id set bit 0 of *status (one int32 on the device that the caller zeroes once
- * and q6w_workspace_status reads; may be NULL). */
+ * followed; query_starts that descend or leave [0, n_tokens] are kept inside
+ * the step's tokens, whose rows are then unspecified.  Such a length, a bad page
+ * id and such starts set bit 0 of *status (one int32 on the device that the
+ * caller zeroes once and q6w_workspace_status reads; may be NULL). */
 typedef struct q6w_paged_batch {
   void* k_pages;
   void* v_pages;

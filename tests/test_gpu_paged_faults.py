@@ -93,3 +93,27 @@ def test_prefix_wait_runs_out(new, kv):
     c = make(n, 8, 2, 64, 16, kv, [40 * i for i in range(n)], [new] * n, seed=7, prefix=3000)
     share = check_stalled(c, [(t, h) for t in range(n * new) for h in range(4)])
     assert share < 0.75
+
+
+@pytest.mark.parametrize("starts,bad", [([0, 4, 8, 12], False), ([2, 2, 5, 11], False), ([0, 8, 4, 12], True),
+                                        ([0, 4, 8, 13], True), ([-1, 4, 8, 12], True), ([9, 4, 8, 12], True),
+                                        ([0, 4, 1 << 30, 12], True), ([0, 4, 8, -5], True)])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_starts_that_cannot_be_are_flagged(starts, bad, prefix):
+    """Kept inside the step's tokens by both calls, and reported."""
+    c = make(3, 8, 2, 64, 16, torch.float32, [20, 3, 40], [4, 4, 4], prefix=prefix)
+    c["starts"] = torch.tensor(starts, dtype=torch.int32).cuda()
+    cos, sin = (torch.ones(100, 32, device="cuda") for _ in range(2))
+    k = torch.randn(12, 2, 64, device="cuda")
+    calls = [lambda st: ops.paged_append(c["q"], k, k, cos, sin, c["kp"], c["vp"], c["table"], c["lens"], c["starts"],
+                                         status=st),
+             lambda st: attend(c, status=st)]
+    for call in calls:
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(status)
+        if bad:
+            with pytest.raises(Q6WError):
+                ops.check_status(status)
+        else:
+            ops.check_status(status)
+        call(None)

@@ -127,33 +127,37 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int tpt = 1 << a.tpt_shift, me = threadIdx.x & (tpt - 1);
   const int t = (blockIdx.x * (256 >> a.tpt_shift) + (threadIdx.x >> a.tpt_shift)) * GROUP;
-  if (t >= a.b.T) return;  // warp-uniform: tpt >= 32
-  const int units = a.hd >> 3;  // eight-element units of a head
-  const int nq = a.H * units, nk = a.b.kv_heads * units, all = nq + 2 * nk;
-  Unit x[GROUP];
+  if (t < a.b.T) {  // warp-uniform: tpt >= 32
+    const int units = a.hd >> 3;  // eight-element units of a head
+    const int nq = a.H * units, nk = a.b.kv_heads * units, all = nq + 2 * nk;
+    Unit x[GROUP];
 #pragma unroll
-  for (int g = 0; g < GROUP; ++g)
-    if (me < all && t + g < a.b.T) x[g] = load_unit(a, t + g, me, nq, nk);
-  int s = token_seq(a.b, t, lane), t0 = 0, t1 = 0;
-  if (s >= 0 && s < a.b.n) seq_tokens(a.b, s, t0, t1);
-  if (GROUP > 1) {
+    for (int g = 0; g < GROUP; ++g)
+      if (me < all && t + g < a.b.T) x[g] = load_unit(a, t + g, me, nq, nk);
+    int s = token_seq(a.b, t, lane), t0 = 0, t1 = 0;
+    if (s >= 0 && s < a.b.n) seq_tokens(a.b, s, t0, t1);
+    if (GROUP > 1) {
 #pragma unroll
-    for (int g = 0; g < GROUP; ++g) {
-      if (t + g >= a.b.T) break;
-      if (g > 0) follow(a.b, t + g, s, t0, t1);
-      const Place p = place_of(a, t + g, s, t0, t1);
-      if (me < all) finish_unit<HALF>(a, t + g, me, nq, nk, p, x[g]);
-    }
-  } else {
-    const Place p = place_of(a, t, s, t0, t1);
-    for (int i = me; i < all;) {
-      Unit v = x[0];
-      const int cur = i;
-      i += tpt;
-      if (i < all) x[0] = load_unit(a, t, i, nq, nk);
-      finish_unit<HALF>(a, t, cur, nq, nk, p, v);
+      for (int g = 0; g < GROUP; ++g) {
+        if (t + g >= a.b.T) break;
+        if (g > 0) follow(a.b, t + g, s, t0, t1);
+        const Place p = place_of(a, t + g, s, t0, t1);
+        if (me < all) finish_unit<HALF>(a, t + g, me, nq, nk, p, x[g]);
+      }
+    } else {
+      const Place p = place_of(a, t, s, t0, t1);
+      for (int i = me; i < all;) {
+        Unit v = x[0];
+        const int cur = i;
+        i += tpt;
+        if (i < all) x[0] = load_unit(a, t, i, nq, nk);
+        finish_unit<HALF>(a, t, cur, nq, nk, p, v);
+      }
     }
   }
+  if (a.b.starts && a.b.status)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.b.n; i += (int64_t)gridDim.x * 256)
+      check_tokens(a.b, (int)i);
 }
 
 // ---- host ------------------------------------------------------------------------

@@ -57,6 +57,12 @@ __device__ __forceinline__ void seq_tokens(const Batch& b, int s, int& t0, int& 
   t1 = min(max(__ldg(b.starts + s + 1), t0), b.T);
 }
 
+// Flags starts of sequence s that descend or leave [0, T].
+__device__ __forceinline__ void check_tokens(const Batch& b, int s) {
+  const int t0 = __ldg(b.starts + s), t1 = __ldg(b.starts + s + 1);
+  if (t0 < 0 || t1 < t0 || t1 > b.T) flag(b.status, kErrInput);
+}
+
 // Sequence of query token t, by the whole warp (all lanes the same t): the
 // last s with starts[s] <= t, found 32-fold a round.  -1 or n: no sequence.
 __device__ __forceinline__ int token_seq(const Batch& b, int t, int lane) {

@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(1024) line_kernel(TcArgs a, int64_t* line) {
     int64_t u = 0;
     if (s < a.b.n) {
       if (__ldg(a.b.lengths + s) > a.b.max_len) flag(a.b.status, kErrInput);
+      check_tokens(a.b, s);
       w.p.s = s;
       w.sequence();
       const int nb = w.blocks();

@@ -367,7 +367,8 @@ def paged_append(queries, keys, values, cos, sin, key_pages, value_pages, page_t
     they were).
 
     ``status``: int32 [1] on the device, zeroed once; bit 0 is set when a
-    length, page id or position is out of range (``check_status``).
+    length, page id or position is out of range or ``query_starts`` descends
+    or leaves [0, T] (``check_status``).
     """
     T = keys.shape[0]
     batch, dev, kv_heads, hd = _paged_batch(key_pages, value_pages, page_table, lengths, query_starts, status, T)
