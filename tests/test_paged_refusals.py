@@ -134,3 +134,14 @@ def test_stall_diagnostic_arguments():
     stall = _lib.load().q6w_selftest_paged_stall
     assert stall(-1) == _lib.Q6W_ERR_ARG and stall((1 << 31) + 1) == _lib.Q6W_ERR_ARG
     assert stall(0) == _lib.Q6W_OK
+
+
+def test_workspace_of_refused_calls_is_0():
+    """What the attention calls refuse by shape has no workspace."""
+    size = _lib.load().q6w_paged_workspace_bytes
+    small = dict(head_dim=16, head_stride=16, slot_stride=64, page_stride=64)
+    assert size(batch(**small, page_size=1), 3, 8, 0) == 0
+    assert size(batch(**small, page_size=2), 3, 8, 0) > 0
+    assert size(batch(**small, page_size=2, kv_dtype=1), 3, 8, 0) == 0
+    many = dict(kv_heads=1, head_dim=16, slot_stride=16, page_stride=256, head_stride=16, query_starts=P)
+    assert size(batch(**many), 1 << 24, 128, 0) == 0 < size(batch(**many), 1 << 24, 127, 0)

@@ -212,10 +212,20 @@ static int32_t check_batch(const char* who, const q6w_paged_batch* p, int32_t n_
   return Q6W_OK;
 }
 
-static int32_t check_heads(const char* who, const q6w_paged_batch* p, int32_t n_heads, Batch* b) {
+// The batch and what else the attention calls are given beside their tensors.
+static int32_t check_attention(const char* who, const q6w_paged_batch* p, int32_t n_tokens, int32_t n_heads,
+                               int32_t prefix_length, Batch* b) {
+  const int32_t st = check_batch(who, p, n_tokens, b);
+  if (st) return st;
   if (n_heads < 1 || n_heads > (1 << 14) || n_heads % p->kv_heads)
     return fail(Q6W_ERR_ARG, "%s: %d query heads are not a multiple of %d kv heads", who, n_heads, p->kv_heads);
   b->rep = n_heads / p->kv_heads;
+  if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
+  if (p->page_size * p->head_dim * (p->kv_dtype == Q6W_KV_F16 ? 2 : 4) < 128)
+    return fail(Q6W_ERR_ARG, "%s: a kv head's part of a page must be at least 128 bytes", who);
+  // row numbers, rounded up to whole tiles, are 32-bit in the kernels
+  if ((int64_t)n_tokens * n_heads > INT32_MAX - 512)
+    return fail(Q6W_ERR_ARG, "%s: %d tokens of %d heads are more rows than 32 bits count", who, n_tokens, n_heads);
   return Q6W_OK;
 }
 
@@ -267,16 +277,8 @@ static int32_t attention(const char* who, const q6w_paged_batch* p, const int32_
                          int32_t zero_padding, void* workspace, size_t workspace_bytes, q6w_stream_t stream) {
   clear_error();
   Batch b;
-  int32_t st = check_batch(who, p, n_tokens, &b);
+  int32_t st = check_attention(who, p, n_tokens, n_heads, prefix_length, &b);
   if (st) return st;
-  st = check_heads(who, p, n_heads, &b);
-  if (st) return st;
-  if (prefix_length < 0 || prefix_length > (1 << 30)) return fail(Q6W_ERR_ARG, "%s: bad prefix_length", who);
-  if (p->page_size * p->head_dim * (p->kv_dtype == Q6W_KV_F16 ? 2 : 4) < 128)
-    return fail(Q6W_ERR_ARG, "%s: a kv head's part of a page must be at least 128 bytes", who);
-  // row numbers, rounded up to whole tiles, are 32-bit in the kernels
-  if ((int64_t)n_tokens * n_heads > INT32_MAX - 512)
-    return fail(Q6W_ERR_ARG, "%s: %d tokens of %d heads are more rows than 32 bits count", who, n_tokens, n_heads);
   if (n_tokens == 0) return Q6W_OK;
   if (!queries || !output || (prefix_length > 0 && !prefix_pages)) return fail(Q6W_ERR_ARG, "%s: null pointer", who);
   if (!aligned(queries, 16) || !aligned(output, 16) || query_stride % 4)
@@ -406,10 +408,7 @@ extern "C" int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_toke
 extern "C" size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
                                             int32_t prefix_length) {
   paged::Batch b;
-  if (paged::check_batch("q6w_paged_workspace_bytes", batch, n_tokens, &b) ||
-      paged::check_heads("q6w_paged_workspace_bytes", batch, n_heads, &b) || prefix_length < 0 ||
-      prefix_length > (1 << 30))
-    return 0;
+  if (paged::check_attention("q6w_paged_workspace_bytes", batch, n_tokens, n_heads, prefix_length, &b)) return 0;
   paged::Regions r;
   return paged::layout(b, batch->head_dim, n_heads, batch->kv_dtype == Q6W_KV_F16, prefix_length, nullptr, &r);
 }
