@@ -7,6 +7,7 @@ include/q6w_b200.h); it links only the CUDA runtime, no torch.
 """
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -28,6 +29,25 @@ def nvcc():
     return path
 
 
+# Kernels that divide their registers among warps (csrc/paged_tc.cu), by their part of
+# the mangled name: a thread's number at launch, which the division needs exactly.
+SPLIT_REGISTERS = {"5paged11rows_kernelI": 128}
+
+
+def check_split_registers(log):
+    """Raise if ptxas gave a kernel of SPLIT_REGISTERS another number of registers
+    than its division needs (the library would refuse its calls)."""
+    kernel = None
+    for line in log.splitlines():
+        entry = re.search(r"Compiling entry function '(\w+)'", line)
+        if entry:
+            kernel = entry.group(1)
+        used = re.search(r"Used (\d+) registers", line)
+        for name, need in SPLIT_REGISTERS.items():
+            if used and kernel and name in kernel and int(used.group(1)) != need:
+                raise RuntimeError(f"{kernel} was compiled to {used.group(1)} registers a thread, its warps divide {need}")
+
+
 def build(verbose=False, jobs=None):
     inc = ["-I", str(ROOT / "include"), "-I", str(HERE / "csrc")]
     objs = []
@@ -45,6 +65,7 @@ def build(verbose=False, jobs=None):
         if p.returncode != 0:
             sys.stderr.write(out)
             raise RuntimeError(f"nvcc failed on {src}")
+        check_split_registers(out)
         objs.append(str(obj))
     link = [nvcc(), *ARCH, "-shared", "-o", str(OUT), *objs, "-lcudart"]
     subprocess.run(link, check=True)

@@ -1103,7 +1103,7 @@ struct TcLaunch {
     {
       std::lock_guard<std::mutex> lock(mu);
       if (!granted[dev & 63]) {
-        // the register split needs all that it divides
+        // the register split needs all that it divides (build.py checks it too)
         cudaFuncAttributes attr;
         Q6W_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
         if (attr.numRegs != S::REGS)
