@@ -145,3 +145,8 @@ def test_workspace_of_refused_calls_is_0():
     assert size(batch(**small, page_size=2, kv_dtype=1), 3, 8, 0) == 0
     many = dict(kv_heads=1, head_dim=16, slot_stride=16, page_stride=256, head_stride=16, query_starts=P)
     assert size(batch(**many), 1 << 24, 128, 0) == 0 < size(batch(**many), 1 << 24, 127, 0)
+
+
+def test_check_status_refuses_the_cpu():
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.check_status(torch.zeros(1, dtype=torch.int32))

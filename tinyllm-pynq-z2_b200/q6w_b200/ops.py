@@ -442,4 +442,7 @@ def _paged_attention(queries, key_pages, value_pages, prefix_pages, prefix_lengt
 
 def check_status(status):
     """Synchronise and raise Q6WError if a paged call set ``status`` (then clear it)."""
-    _lib.check(_on_device(status.get_device(), _lib.load().q6w_workspace_status, status.data_ptr()), "paged cache")
+    dev = status.get_device()
+    if dev < 0 or status.dtype is not _I32 or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor on a CUDA device")
+    _lib.check(_on_device(dev, _lib.load().q6w_workspace_status, status.data_ptr()), "paged cache")
