@@ -164,3 +164,33 @@ def test_keys_that_are_not_finite(value, H, KV, hd, ps, kv):
     hit = {(i, g) for i, g, _ in struck}
     clean = torch.tensor([[(i, g) not in hit for g in range(KV)] for i in range(len(lens))]).repeat_interleave(H // KV, 1)
     assert bool(got[clean.cuda()].isfinite().all())
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (5, 0), (1, 12), (5, 11)])
+def test_every_operand_keeps_its_bits(new, prefix, hd, kv):
+    """Scores of one product and outputs of one product, of operands with full
+    significands: a query and a key of two (FP32 pages) parts err by 4 u each, the
+    parts' products, their sum, the scale and the exponent by 4 u: 12 u A.  Outputs:
+    2 delta, the parts of weight and value 8 u, the sum of N <= 16 weights and the
+    quotient, and a join, 32 u.  Operands of 16 bits would miss it by 128 u."""
+    N = 16
+    c = make(3, 8, 2, hd, 16, kv, [N - prefix - new] * 3, [new] * 3, seed=hd, prefix=prefix)
+    g = torch.Generator().manual_seed(2)
+    keys = torch.zeros(N, hd)
+    keys[:, 1] = torch.rand(N, generator=g) - 0.5
+    values = torch.zeros(N, hd)
+    values[range(N), range(N)] = torch.rand(N, generator=g) + 0.5
+    keys, values = keys.to(kv).float(), values.to(kv).float()
+    fill(c, keys.cuda(), values.cuda())
+    x = math.sqrt(hd) * (torch.rand(8, generator=g) + 0.5)
+    c["q"].zero_()
+    c["q"][..., 1] = x.cuda()
+    scores = x.double()[:, None] * keys[None, :, 1].double() / math.sqrt(hd)
+    got = attend(c).double().cpu()
+    want, _ = softmax64(c, scores, values)
+    A = float(scores.abs().max())
+    assert not got[want == 0].any()
+    err = ((got - want).abs() / want.clamp(min=1e-300)).masked_fill(want == 0, 0.0)
+    assert float(err.max()) <= (2 * 12 * A + 8 + 32) * U

@@ -117,3 +117,37 @@ def test_starts_that_cannot_be_are_flagged(starts, bad, prefix):
         else:
             ops.check_status(status)
         call(None)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("H,KV,hd,ps", [(8, 4, 16, 8), (8, 2, 64, 1), (8, 2, 64, 16), (10, 2, 128, 64)])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("at", [0, 24, 200, 349, 399])
+def test_a_bad_page_anywhere_spoils_the_rows_that_meet_it(at, new, H, KV, hd, ps, kv):
+    """In a unit that every row sees whole, in a later one, in the second tile of a unit, behind some rows' positions."""
+    c = make(3, H, KV, hd, ps, kv, [400 - new] * 3, [new] * 3, seed=at)
+    want = attend(c)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for bad in (-1, c["kp"].shape[0], 1 << 30):
+        c["table"][1, at // ps] = bad
+        got = attend(c, status=status)
+        first = max(0, at // ps * ps - (400 - new))  # rows in front of the page's first position see nothing of it
+        spoilt = slice(new + first, 2 * new)
+        assert bool(got[spoilt].isnan().all())
+        keep = torch.ones(3 * new, dtype=torch.bool)
+        keep[spoilt] = False
+        assert torch.equal(got[keep], want[keep])
+        with pytest.raises(Q6WError):
+            ops.check_status(status)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("at", [0, 130, 299])
+def test_a_bad_prefix_page_spoils_every_row(at, new, kv):
+    c = make(3, 8, 2, 64, 16, kv, [40, 0, 300], [new] * 3, prefix=300)
+    c["prefix_pages"][at // 16] = c["kp"].shape[0]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert bool(attend(c, status=status).isnan().all())
+    with pytest.raises(Q6WError):
+        ops.check_status(status)
