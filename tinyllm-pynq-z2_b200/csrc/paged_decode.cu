@@ -125,7 +125,7 @@ struct DecodeMaps {
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 
-// The line of units: prefix sums over 256 stretches of sequences.
+// The line of units: prefix sums over 128 stretches of sequences.
 struct Line {
   int64_t pref[kDecodeThreads];
   int64_t total;
@@ -843,8 +843,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
 // pieces' weights, then groups of heads head_dim / 4 threads share the pieces out.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeMost = 1024;  // pieces of an item: the CTAs of a grid
-
 constexpr int kFewPieces = 8;
+constexpr int kMergeWeights = kMergeMost > 8 * kFewPieces ? kMergeMost : 8 * kFewPieces;
 
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
   grid_dep_wait();  // (launched as the decode kernel drains)
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
   block_heads(a, d.y, h0, nr);
   const int r0 = blockIdx.y, heads = d.z <= kFewPieces ? nr : 1;
   if (r0 >= nr || (heads > 1 && r0 > 0)) return;
-  __shared__ float w[kMergeMost * 8], total[8], top[8];
+  __shared__ float w[kMergeWeights], total[8], top[8];
   __shared__ float4 so[kMergeThreads];
   const int STATE = state_floats(a.hd), hd = a.hd, M0 = 8 * hd + r0, L0 = 8 * hd + 8 + r0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -886,40 +886,34 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
     }
   }
   __syncthreads();
-  const int per = heads * hd / 4, groups = max(1, kMergeThreads / per);  // (per may exceed the block: 8 heads of 128)
+  const int per = heads * hd / 4, groups = kMergeThreads / per;  // 4 to 256 threads a group
   const int64_t row = (int64_t)d.x * a.H + h0 + r0;
-  for (int x0 = 0; x0 < per; x0 += kMergeThreads) {
-    const int x = x0 + tid % min(per, kMergeThreads), grp = groups > 1 ? tid / per : 0, r = 4 * x / hd;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (grp < groups && x < per) {
+  const int x = tid % per, grp = tid / per, r = 4 * x / hd;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
 #pragma unroll 4
-      for (int k = grp; k < d.z; k += groups) {
-        const float4 v = *reinterpret_cast<const float4*>(piece(k) + r0 * hd + 4 * x);
-        const float p = w[k * heads + r];
-        o.x = fmaf(p, v.x, o.x);
-        o.y = fmaf(p, v.y, o.y);
-        o.z = fmaf(p, v.z, o.z);
-        o.w = fmaf(p, v.w, o.w);
-      }
-    }
-    if (groups > 1) {
-      so[tid] = o;
-      __syncthreads();
-      if (grp == 0)
-        for (int k = 1; k < groups; ++k) {
-          const float4 v = so[k * per + tid];
-          o.x += v.x;
-          o.y += v.y;
-          o.z += v.z;
-          o.w += v.w;
-        }
-    }
-    if (grp == 0 && x < per) {
-      const float l = total[r], inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-      *reinterpret_cast<float4*>(a.out + row * hd + 4 * x) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-      if (a.state && 4 * x == r * hd) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(top[r], l);
+    for (int k = grp; k < d.z; k += groups) {
+      const float4 v = *reinterpret_cast<const float4*>(piece(k) + r0 * hd + 4 * x);
+      const float p = w[k * heads + r];
+      o.x = fmaf(p, v.x, o.x);
+      o.y = fmaf(p, v.y, o.y);
+      o.z = fmaf(p, v.z, o.z);
+      o.w = fmaf(p, v.w, o.w);
     }
   }
+  so[tid] = o;
+  __syncthreads();
+  if (grp > 0) return;
+  for (int k = 1; k < groups; ++k) {
+    const float4 v = so[k * per + tid];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
+  }
+  const float l = total[r], inv = a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+  *reinterpret_cast<float4*>(a.out + row * hd + 4 * x) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (a.state && 4 * x == r * hd) *reinterpret_cast<float2*>(a.state + (row + r) * 2) = make_float2(top[r], l);
 }
 
 // ---- host ---------------------------------------------------------------------
