@@ -238,6 +238,17 @@ template <int KU>
 struct Cursor {
   int64_t x, x1, first;
   int s, block, keys, us, u0, u1, key0, key1;
+  // At unit x_ of the line, up to x1_.
+  __device__ __forceinline__ void begin(const Batch& b, const Line& line, int64_t x_, int64_t x1_, int KVB, int lane) {
+    x = x_;
+    x1 = x1_;
+    find_seq<KU>(b, line, muldiv(x, 1, KVB), lane, s, first);
+    keys = keys_of(b, s);
+    us = units_of<KU>(keys);
+    block = (int)muldiv(x - first * KVB, 1, us);
+    u0 = (int)(x - first * KVB - (int64_t)block * us);
+    piece();
+  }
   __device__ __forceinline__ void piece() {
     u1 = (int)min((int64_t)us, u0 + (x1 - x));
     key0 = u0 * KU;
@@ -306,13 +317,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// The larger of two values, NaN if either is.
-__device__ __forceinline__ float max_nan(float x, float y) {
-  float z;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-  return z;
-}
-
 // x = hi + lo as TF32 operands: hi rounded to nearest (11 bits), lo the exact
 // rest, of which the MMA takes the upper 11 bits.  A NaN stays one in lo.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
@@ -328,21 +332,100 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// q . K of one row of a tile in shared memory, one FP32 product after the other; the
-// kv head's elements start at element `first` of the row.
+// The line's units and the warps that share them: few units are spread over the
+// CTAs first, over a CTA's warps second.
+struct Workers {
+  int64_t units, count, me;
+  int aw;  // warps of a CTA that take part
+  __device__ __forceinline__ explicit Workers(int64_t n) : units(n) {
+    const int warp = threadIdx.x >> 5;
+    aw = units >= (int64_t)gridDim.x * kDecodeWarps ? kDecodeWarps : (int)(((uint32_t)units + gridDim.x - 1) / gridDim.x);
+    count = min((int64_t)gridDim.x * aw, units);
+    me = warp < aw ? (int64_t)blockIdx.x * aw + warp : count;
+  }
+  __device__ __forceinline__ bool active() const { return me < count; }
+  __device__ __forceinline__ int64_t begin() const { return muldiv(me, units, count); }
+  __device__ __forceinline__ int64_t end() const { return muldiv(me + 1, units, count); }
+};
+
+// The state of a piece in FP32, one product after the other.  A page out of range leaves NaN.
+template <typename KT>
+__device__ void plain_piece(const DecodeArgs& a, int s, int h0, int nr, int key0, int key1, bool whole,
+                                         float* slot) {
+  const Batch& b = a.b;
+  const int lane = threadIdx.x & 31;
+  for (int n = 0; n < nr; ++n) {
+    const int h = h0 + n;
+    const float* q = a.q + s * a.ldq + (int64_t)h * a.hd;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int key = key0; key < key1; ++key) {
+      const int id = __ldg(b.table + s * b.table_stride + (key >> b.shift));
+      if ((unsigned)id >= (unsigned)b.n_pages) {
+        l = NAN;
+        break;
+      }
+      const int64_t at = id * b.page_stride + (key & ((1 << b.shift) - 1)) * b.slot_stride + h / b.rep * b.head_stride;
+      const KT* k = static_cast<const KT*>(b.k) + at;
+      const KT* v = static_cast<const KT*>(b.v) + at;
+      float x = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 32 * e < a.hd) x = fmaf(__ldg(q + lane + 32 * e), (float)k[lane + 32 * e], x);
+#pragma unroll
+      for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+      x *= a.scale;
+      const float f = x > m ? ex2(m - x) : 1.f, p = ex2(x - ref_of(x > m ? x : m));
+      if (x > m) m = x;
+      l = fmaf(l, f, p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 32 * e < a.hd) o[e] = fmaf(p, (float)v[lane + 32 * e], o[e] * f);
+    }
+    const int64_t row = (int64_t)s * a.H + h;
+    const float inv = !whole || a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+    float* dst = whole ? a.out + row * a.hd : slot + n * a.hd;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < a.hd) dst[lane + 32 * e] = o[e] * inv;
+    if (lane == 0 && !whole) {
+      slot[8 * a.hd + n] = m;
+      slot[8 * a.hd + 8 + n] = l;
+    } else if (lane == 0 && a.state) {
+      *reinterpret_cast<float2*>(a.state + row * 2) = make_float2(m, l);
+    }
+  }
+}
+
+// Goes over a warp's stretch once more and makes the pieces anew whose sum of weights
+// is not a number.  That may be another kv head's doing (its infinite key times this
+// head's zeros in the MMA) or the parts' (inf - inf); here a key's score is its own,
+// and one of -inf is a weight of 0.
 template <int HDF, typename KT>
-__device__ __noinline__ float plain_score(const float* q, const uint8_t* tile, int row, int first, int hd) {
-  using S = DecodeShape<HDF, KT>;
-  float dot = 0.f;
-#pragma unroll 1
-  for (int d = 0; d < hd; ++d)
-    dot = fmaf(__ldg(q + d), (float)*reinterpret_cast<const KT*>(tile + S::place(row, (first + d) * S::ES)), dot);
-  return dot;
+__device__ __noinline__ void plain_pieces(const DecodeArgs& a, const Line& line) {
+  const Batch& b = a.b;
+  const int lane = threadIdx.x & 31, KVB = b.kv_heads / a.F * a.HB, STATE = state_floats(a.hd);
+  const Workers k(line.total * KVB);
+  if (!k.active()) return;
+  float* slots = a.wpart + ((size_t)blockIdx.x * kDecodeWarps + (threadIdx.x >> 5)) * 2 * STATE;
+  Cursor<DecodeShape<HDF, KT>::KU> cur;
+  cur.begin(b, line, k.begin(), k.end(), KVB, lane);
+  const int64_t x = cur.x;
+  while (cur.x < cur.x1) {
+    int h0, nr;
+    block_heads(a, cur.block, h0, nr);
+    const bool whole = cur.u0 == 0 && cur.u1 == cur.us;
+    float* slot = slots + (cur.x == x ? 0 : 1) * STATE;
+    const int64_t row = (int64_t)cur.s * a.H + h0 + lane;
+    float l = 0.f;
+    if (lane < nr) l = !whole ? slot[8 * a.hd + 8 + lane] : a.state ? a.state[row * 2 + 1] : a.out[row * a.hd];
+    if (__any_sync(0xffffffffu, l != l)) plain_piece<KT>(a, cur.s, h0, nr, cur.key0, cur.key1, whole, slot);
+    cur.next(b, KVB);
+  }
 }
 
 template <int HDF, typename KT>
 __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
-    decode_kernel(DecodeArgs a, const __grid_constant__ DecodeMaps maps) {
+    decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ DecodeMaps maps) {
   using S = DecodeShape<HDF, KT>;
   constexpr bool kHalf = std::is_same<KT, __half>::value;
   constexpr int NK = S::NK, NVC = S::NVC, EK = S::EK, EV = S::EV, CK = S::CK, CV = S::CV, STG = S::STG;
@@ -356,6 +439,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   __shared__ uint64_t bars[kDecodeWarps * STG];
   __shared__ Line line;
   __shared__ Seg segs[2 * kDecodeWarps];
+  __shared__ int odd;  // a sum of weights was not a number
   const Batch& b = a.b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;  // the MMA fragments' row group and column group
@@ -365,6 +449,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   const int hd_shift = 31 - __clz(a.hd);
   uint64_t* bar = bars + warp * STG;
   if (threadIdx.x == 0) {
+    odd = 0;
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
   }
@@ -372,25 +457,13 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   fence_mbar_init();
   build_line<S::KU>(b, line);
   const int KVB = b.kv_heads / a.F * a.HB;
-  const int64_t units = line.total * KVB;
-  // few units: spread them over the CTAs first, over a CTA's warps second
-  const int aw = units >= (int64_t)gridDim.x * kDecodeWarps ? kDecodeWarps : (int)(((uint32_t)units + gridDim.x - 1) / gridDim.x);
-  const int64_t workers = min((int64_t)gridDim.x * aw, units);
-  const int64_t wi = (int64_t)blockIdx.x * aw + warp;
-  const bool active = warp < aw && wi < workers;
+  const Workers work(line.total * KVB);
   if (lane < 2) segs[2 * warp + lane].valid = 0;
   float* slots = a.wpart + ((size_t)blockIdx.x * kDecodeWarps + warp) * 2 * STATE;
-  if (active) {
+  if (work.active()) {
     Cursor<S::KU> cur;
-    cur.x = muldiv(wi, units, workers);
-    cur.x1 = muldiv(wi + 1, units, workers);
+    cur.begin(b, line, work.begin(), work.end(), KVB, lane);
     const int64_t xb = cur.x;
-    find_seq<S::KU>(b, line, muldiv(cur.x, 1, KVB), lane, cur.s, cur.first);
-    cur.keys = keys_of(b, cur.s);
-    cur.us = units_of<S::KU>(cur.keys);
-    cur.block = (int)muldiv(cur.x - cur.first * KVB, 1, cur.us);
-    cur.u0 = (int)(cur.x - cur.first * KVB - (int64_t)cur.block * cur.us);
-    cur.piece();
 
     // ---- loads
     const uint32_t ring = ((smem_u32(smem_raw) + 1023) & ~1023u) + warp * S::RING;
@@ -581,35 +654,14 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
           }
         }
         // ---- the references, when a score passes them by too much
-        float m0 = max_nan(x[0][0], x[0][2]), m1 = max_nan(x[0][1], x[0][3]);
+        float m0 = fmaxf(x[0][0], x[0][2]), m1 = fmaxf(x[0][1], x[0][3]);
         if constexpr (NT == 2) {
-          m0 = max_nan(m0, max_nan(x[1][0], x[1][2]));
-          m1 = max_nan(m1, max_nan(x[1][1], x[1][3]));
+          m0 = fmaxf(m0, fmaxf(x[1][0], x[1][2]));
+          m1 = fmaxf(m1, fmaxf(x[1][1], x[1][3]));
         }
         m0 *= sc0;
         m1 *= sc1;
-        if (__any_sync(kAll, !(m0 - ref0 <= kLimit && m1 - ref1 <= kLimit))) {
-          // A score that is not a number may be another kv head's doing (its infinite
-          // key times this head's zeros), or the parts' (inf - inf): it is computed again
-          // from the tile, unless a page was missing.
-          const int st = stage == 0 ? STG - 1 : stage - 1;
-          m0 = m1 = -INFINITY;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int n = 2 * c + (i & 1);
-              if (x[t][i] != x[t][i] && n < nr && !(bad >> (2 * st + t) & 1)) {
-                const float dot = plain_score<HDF, KT>(a.q + s * a.ldq + (int64_t)(h0 + n) * a.hd,
-                                                       ring_g + st * S::HALF + t * S::TILE, krow + 8 * (i >> 1),
-                                                       fc[i & 1] * a.hd, a.hd);
-                x[t][i] = kHalf ? dot * (a.scale / (i & 1 ? sc1 : sc0)) : dot;
-              }
-              if (i & 1) m1 = fmaxf(m1, x[t][i]); else m0 = fmaxf(m0, x[t][i]);
-            }
-          }
-          m0 *= sc0;
-          m1 *= sc1;
+        if (__any_sync(kAll, m0 - ref0 > kLimit || m1 - ref1 > kLimit)) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(kAll, m0, o));
@@ -715,6 +767,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
         l0 += __shfl_xor_sync(kAll, l0, o);
         l1 += __shfl_xor_sync(kAll, l1, o);
       }
+      if (l0 != l0 || l1 != l1) odd = 1;
       if (late) l0 = l1 = NAN;
       const bool begin = cur.u0 == 0, end = cur.u1 == cur.us, whole = begin && end;
       const int which = cur.x == xb ? 0 : 1;
@@ -766,6 +819,10 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
   }
   grid_dep_launch();
   __syncthreads();
+  if (odd) {
+    plain_pieces<HDF, KT>(a, line);
+    __syncthreads();
+  }
   // ---- pieces of items inside this CTA, in order
   if (threadIdx.x == 0) a.desc[blockIdx.x].z = 0;
   const float* pieces = a.wpart + (size_t)blockIdx.x * kDecodeWarps * 2 * STATE;
@@ -829,7 +886,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
       // the CTA that holds the item's last unit
       const int us = units_of<S::KU>(keys_of(b, f.s));
       const int64_t lastu = f.first * KVB + (int64_t)(f.block + 1) * us - 1;
-      const int c1 = (int)(owner_of(lastu, units, workers) / aw);
+      const int c1 = (int)(owner_of(lastu, work.units, work.count) / work.aw);
       a.desc[blockIdx.x] = make_int4(f.s, f.block, c1 - (int)blockIdx.x + 1, 0);
     }
     i = j;
@@ -844,7 +901,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeShape<HDF, KT>::CTAS)
 constexpr int kMergeThreads = 256;
 constexpr int kMergeMost = 1024;  // pieces of an item: the CTAs of a grid
 constexpr int kFewPieces = 8;
-constexpr int kMergeWeights = kMergeMost > 8 * kFewPieces ? kMergeMost : 8 * kFewPieces;
+// (kMergeMost floats would do.  With 4 KB instead of 32 more of these blocks wait beside
+// the decode kernel's last CTAs: 256 requests of up to 512 keys, hd 64, 51.2 us against 50.0.)
+constexpr int kMergeWeights = 8 * kMergeMost;
 
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(DecodeArgs a) {
   grid_dep_wait();  // (launched as the decode kernel drains)

@@ -766,7 +766,9 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       return mine;
     };
     uint32_t sn = 0, s_seen[2] = {0, 0}, done = 0;
-    bool ok = true;  // false: a wait ran out, and the rows of this and all later pieces become NaN
+    // (false: a wait ran out.  Later ones return at once, and the rows of this and all
+    // later pieces become NaN.)
+    bool ok = true;
     for (; w.more(); w.next()) {
       if (TILES == 2 && t == 1 && w.rows() <= 128) continue;
       const int ri = w.p.j * S::ROWS + t * 128 + r;  // row of the (sequence, kv head)
@@ -775,7 +777,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
       const int64_t token = w.p.tok0 + tok;
       const int vis = in ? w.seen(tok) : 0;
       float sc = a.scale;
-      if (ok) {
+      {
         // Q's parts into tensor memory, two elements a column
         const float* qp = a.q + token * a.ldq + (int64_t)h * HD;
         float scale = 1.f;
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
 #pragma unroll
       for (int d = 0; d < MYD; ++d) acc[d] = 0.f;
       float ref = kUnseen, l = 0.f;
-      for (int u = ok ? w.p.u0 : w.p.u1; u < w.p.u1; ++u) {
+      for (int u = w.p.u0; u < w.p.u1; ++u) {
         const int buf = TILES == 2 ? t : (int)(sn & 1);
         ok = wait(s_full + buf, s_seen[buf]++ & 1) && ok;
         if (HALVES == 1) {
