@@ -404,7 +404,7 @@ typedef struct q6w_paged_batch {
  * nothing, neither do positions at or beyond rope_len (which set status
  * bit 0); their rows of rotated are zeroed when zero_padding is set and left
  * as they were otherwise.  A bad page id drops the token's key and value.
- * Two tokens of one call that land in one slot leave either's row. */
+ * Two tokens of one call that land in one slot leave it with parts of either. */
 Q6W_API int32_t q6w_paged_append(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
                                  const float* queries, int64_t query_stride, const float* keys,
                                  int64_t key_stride, const float* values, int64_t value_stride,
@@ -426,14 +426,35 @@ Q6W_API size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n
  * and a prompt's or a chunk's attention for more.  queries (rotated)
  * [n_tokens, n_heads, head_dim] FP32 with a token stride in elements
  * (a multiple of 4); output [n_tokens, n_heads, head_dim] contiguous.
- * n_heads is a multiple of kv_heads, and page_size * head_dim elements are
- * at least 128 bytes.  Scores, softmax and sums are FP32.  A
- * token with no visible key (length 0, padding by length) gives zeros; rows
+ * n_heads is a multiple of kv_heads, n_tokens * n_heads is below 2^31 - 512,
+ * and page_size * head_dim elements are at least 128 bytes (append takes
+ * smaller pages; head dims 256 and 512 of q6w_gqa_attention are not offered).
+ * A token with no visible key (length 0, padding by length) gives zeros; rows
  * of tokens that no sequence holds are zeroed when zero_padding is set and
- * left as they were otherwise.  Slots behind a sequence's length may hold anything.  A row that
- * meets a bad page id is NaN.  workspace: 256-byte aligned,
- * q6w_paged_workspace_bytes; not read before it is written, so it needs no
- * clearing and may be shared by calls of one stream. */
+ * left as they were otherwise.  Slots behind a sequence's length, and in a
+ * chunk later tokens' keys and values, may hold anything.  A row that meets a
+ * bad page id is NaN.
+ *
+ * Numbers.  Scores, softmax statistics and sums are FP32.  FP16 keys and values
+ * enter the products as they are, everything else as parts that keep at least 22
+ * bits.  With FP16 pages these are FP16 numbers: elements of a query
+ * below 2^-17 of its head's largest err by up to 2^-39 of that, weights below
+ * 2^-17 of their row's largest by 2^-39 of it (2^-15 and 2^-37 with
+ * query_starts and over a shared prefix).  With FP32 pages sums of weights up to 1
+ * times values must stay inside FP32's range.  A visible key or value that is
+ * not finite makes NaN of its token's row for the heads of its kv head, in every
+ * dimension, where the formula may leave some of them finite.  For one token a
+ * sequence the sequence's own keys and values follow the formula: a score of
+ * -inf is a weight of 0, a value spoils its dimension alone (FP32 values above
+ * 3.402e38 count as infinite).
+ *
+ * Speed.  NULL query_starts take the kernel for single tokens, bound by reading
+ * keys and values (once for each 8 heads of a kv head), anything else one that
+ * computes tiles of 128 or 256 rows (tokens times heads of a kv head), full or
+ * not: give a step's single tokens and its longer chunks to two calls.
+ *
+ * workspace: 256-byte aligned, q6w_paged_workspace_bytes; not read before it is
+ * written, so it needs no clearing and may be shared by calls of one stream. */
 Q6W_API int32_t q6w_paged_attention(const q6w_paged_batch* batch, int32_t n_tokens, int32_t n_heads,
                                     const float* queries, int64_t query_stride, float* output,
                                     int32_t zero_padding, void* workspace, size_t workspace_bytes,

@@ -59,3 +59,24 @@ def test_chunks_beyond_32_bits(prefix, kv):
     if prefix:
         c["prefix_pages"][0] = pages - 3
     assert torch.equal(attend(c), want)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("prefix", [0, 90])
+def test_a_mixed_step_in_two_calls(prefix, kv):
+    """Single tokens and chunks of one step, each in a call of its own, into slices of one buffer."""
+    from q6w_b200 import ops
+
+    singles, chunks = 12, 3
+    past, new = [i * 31 for i in range(singles)] + [0, 40, 333], [1] * singles + [70, 5, 128]
+    c = make(singles + chunks, 8, 2, 64, 16, kv, past, new, seed=1, prefix=prefix)
+    out = torch.full_like(c["q"], 7.0)
+    for rows, toks, starts in ((slice(0, singles), slice(0, singles), None),
+                               (slice(singles, None), slice(singles, None), c["starts"][singles:] - singles)):
+        args = (c["table"][rows], c["lens"][rows], starts)
+        if prefix:
+            ops.shared_prefix_attention(c["q"][toks], c["kp"], c["vp"], c["prefix_pages"], prefix, *args, out=out[toks])
+        else:
+            ops.paged_attention(c["q"][toks], c["kp"], c["vp"], *args, out=out[toks])
+    check(c, out)
+    check(c, attend(c))
