@@ -15,10 +15,11 @@ namespace paged {
 // every query and key head at the token's position, the value rows copied.
 // Bound by memory: per token 4 (2 H + 2 KV) head_dim bytes of activations and
 // the page rows.  64 chunks of 1-511 tokens with 48 heads of 128, FP16 pages: 737 MB in
-// 118-126 us, 5.8-6.2 TB/s; 2048 prompts of the tiny model (16 heads of 16): 552 MB
-// in 112 us, 4.9 TB/s, the chain search -> length -> page behind it.  `tpt` threads take one token (a whole warp at least, so
-// that the search for the token's sequence is a warp's), eight consecutive
-// elements a thread and step: two 16-byte loads, one or two 16-byte stores.
+// 127-134 us, 5.5-5.8 TB/s; 2048 prompts of the tiny model (16 heads of 16): 552 MB
+// in 113-116 us, 4.8-4.9 TB/s, the chain search -> length -> page behind it (ranges: ten
+// calls in a graph, a call among others).  `tpt` threads take one token (a whole warp
+// at least, so that the search for the token's sequence is a warp's), eight
+// consecutive elements a thread and step: two 16-byte loads, one or two 16-byte stores.
 
 constexpr int kGroup = 4;  // tokens of a thread, narrow tokens
 

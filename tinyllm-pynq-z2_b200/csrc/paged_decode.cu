@@ -19,9 +19,10 @@
 // Precision.  FP16 keys and values are exact operands; queries (scaled by a
 // power of two per head, half_scale) and weights enter as two FP16 parts, hi + lo,
 // 22 bits.  FP32 keys, values, queries and weights enter as two TF32 parts and
-// the products hi hi + hi lo + lo hi, dropping terms of 2^-22.  The MMA adds
-// in FP32; a tile's output is added to o in registers, rounded to nearest, so
-// no long sum lives in the MMA's accumulator.
+// the products hi hi + hi lo + lo hi, dropping terms of 2^-22; the first part of a
+// number above 2^128 (1 - 2^-12) rounds to infinity.  The MMA adds in FP32; a unit's
+// output (16 or 32 keys) is added to o in registers, rounded to nearest, so no long
+// sum lives in the MMA's accumulator.
 //
 // Narrow heads.  While heads of head_dim <= 32 lie side by side in a slot, F kv
 // heads are treated as one of F head_dim dims: their queries stand block-
@@ -30,18 +31,20 @@
 // at full width.
 //
 // Layout of the work.  An item is (sequence, F kv heads, block of up to eight
-// query heads), cut into units of 16 keys.  The units of all items lie on one
+// query heads), cut into units of 16 keys (32 where rows have up to 128 bytes).  More
+// than eight heads a kv head are items of their own that read the keys again (64
+// requests of 128-8192 FP16 keys, heads of 64: 117 us with 8 a kv head, 197 with 16).  The units of all items lie on one
 // line (a prefix sum of the lengths, taken by every CTA for itself), and every
 // warp takes an equal stretch of it: ragged lengths and few long sequences
 // balance alike.  A warp that holds an item whole writes its output; pieces
 // of an item go through the workspace, joined by their CTA when it holds them
 // all, else by merge_kernel.
 //
-// Measured (a call, joins included): 64 requests of 128-16384 keys, FP16, 8 heads a
-// group of 64: 102-107 us for 542 MB, 5.1-5.3 TB/s; 37 requests, FP32, 5 heads a group of
-// 128: 85 us for 380 MB; 8192 requests of 20-147 keys, FP32, heads of 16: 94 us for 357 MB,
-// bound by instruction issue; one request of 32768 keys, FP32: 27 us for 67 MB, of
-// which start-up and joins are about 15.
+// Measured (joins included; ten calls in a graph, a call among others): 64 requests of
+// 128-16384 keys, FP16, 8 heads a group of 64: 102-106 us for 542 MB, 5.1-5.3 TB/s; 37
+// requests, FP32, 5 heads a group of 128: 82-85 us for 380 MB; 8192 requests of 20-147
+// keys, FP32, heads of 16: 95-98 us for 357 MB, bound by instruction issue; one request of
+// 32768 keys, FP32: 27-29 us for 67 MB, of which start-up and joins are about 15.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -26,10 +26,13 @@
 // tiles in a CTA (head_dim <= 64) the softmax of one runs under the MMAs of the
 // other, with one tile (head_dim 128) S has two buffers.  An MMA takes about 60
 // cycles whether N is 64 or 128, so O is one MMA wide where head_dim is 128.
-// Measured: 2 x 2048 tokens behind up to 6144, FP16, 32 heads over 8 kv heads of 128: 825
-// us a call for 344 GFLOP, 416 TFLOP/s; 1024 tokens of 32 heads over 4 kv heads of 64 and
-// 4096 FP32 keys, with their own 20-148 keys: 332 us a call for 35 GFLOP, of which this
-// kernel about 250, each tile behind its chain softmax -> PV -> QK.
+// Measured (ten calls in a graph, a call among others): 2 x 2048 tokens behind up to 6144,
+// FP16, 32 heads over 8 kv heads of 128: 840-890 us for 344 GFLOP, 385-410 TFLOP/s; 1024
+// tokens of 32 heads over 4 kv heads of 64 and 4096 FP32 keys, with their own 20-148
+// keys: 340-350 us for 35 GFLOP, of which this kernel about 265, each tile behind its
+// chain softmax -> PV -> QK (tensor pipe 23% busy).  Blocks of few rows cost as
+// much as full ones: 64 requests with one token each, behind 128-16384 FP16 keys, take
+// 434 us here and 103 in the decode kernel.
 //
 // Roles: eight softmax warps (four a tile; with one tile two threads a row, each
 // half of the keys and of O), four load warps, one MMA warp.
@@ -90,7 +93,10 @@ struct TcShape {
   static constexpr int REGS = 128;
   static constexpr int SOFT_REGS = 160, LOAD_REGS = 96, MMA_REGS = 96;
   static_assert(SOFT * SOFT_REGS + 4 * LOAD_REGS + 4 * MMA_REGS <= (SOFT + 8) * REGS, "register split");
-  static constexpr int kFlush = kHalf ? 4 : 2;  // units between additions of O to registers
+  // Units between additions of O to registers.  FP32, chunks of 201-597 tokens: errors of
+  // 3.4e-7 with every unit, 6.3e-7 with every second (406 against 387 us when it was
+  // chosen), the plain FP32 form 6.2e-7.
+  static constexpr int kFlush = kHalf ? 4 : 2;
   static constexpr size_t SMEM = 1024 + (size_t)STG * 2 * HALF;
 };
 
