@@ -441,12 +441,11 @@ Q6W_API size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n
  * below 2^-17 of its head's largest err by up to 2^-39 of that, weights below
  * 2^-17 of their row's largest by 2^-39 of it (2^-15 and 2^-37 with
  * query_starts and over a shared prefix).  With FP32 pages sums of weights up to 1
- * times values must stay inside FP32's range.  A visible key or value that is
- * not finite makes NaN of its token's row for the heads of its kv head, in every
- * dimension, where the formula may leave some of them finite.  For one token a
- * sequence the sequence's own keys and values follow the formula: a score of
- * -inf is a weight of 0, a value spoils its dimension alone (FP32 values above
- * 3.402e38 count as infinite).
+ * times values must stay inside FP32's range.  Visible keys and values that
+ * are not finite follow the formula: outputs that it makes infinite or NaN come out as
+ * one of these, others keep their numbers (a score of -inf is a weight of 0, a
+ * value spoils its dimension alone); a row whose scores are all -inf is zero.
+ * For one token a sequence FP32 values above 3.402e38 count as infinite.
  *
  * Speed.  NULL query_starts take the kernel for single tokens, bound by reading
  * keys and values (once for each 8 heads of a kv head), anything else one that

@@ -198,3 +198,54 @@ def test_every_operand_keeps_its_bits(new, prefix, hd, kv):
     assert not got[want == 0].any()
     err = ((got - want).abs() / want.clamp(min=1e-300)).masked_fill(want == 0, 0.0)
     assert float(err.max()) <= (2 * 12 * A + 8 + 32) * U
+
+
+def check_definition(c, out):
+    """Every row against softmax over the keys that it sees: NaN and infinities where the
+    definition has them; a head all of whose scores are -inf (0 / 0) is zero, like one without keys."""
+    H, hd = c["q"].shape[1:]
+    KV, ps, P = c["kp"].shape[2], c["kp"].shape[1], c["prefix"]
+    t = 0
+    for i, (a, b) in enumerate(zip(c["past"], c["new"])):
+        at = torch.arange(a + b, device="cuda")
+        pre = torch.arange(P, device="cuda")
+        k, v = (torch.cat((pool[c["prefix_pages"][pre // ps].long(), pre % ps],
+                           pool[c["table"][i, at // ps].long(), at % ps])).double() for pool in (c["kp"], c["vp"]))
+        for j in range(b):
+            N = P + a + j + 1
+            q = c["q"][t].double().unflatten(0, (KV, H // KV))
+            s = torch.einsum("grd,kgd->grk", q, k[:N]) / math.sqrt(hd)
+            w = torch.softmax(s, -1)
+            nothing = (s == -math.inf).all(-1).flatten()
+            want = torch.einsum("grk,kgd->grd", w, v[:N]).flatten(0, 1)
+            want[nothing] = 0.0
+            finite = want.isfinite()
+            plain = lambda x: torch.where(x.isfinite(), x.abs(), 0.0)
+            W = torch.einsum("grk,kgd->grd", torch.nan_to_num(w, nan=0.0), plain(v[:N])).flatten(0, 1)
+            A = torch.einsum("grd,kgd->grk", q.abs(), plain(k[:N])).amax(-1).flatten() / math.sqrt(hd)
+            tol = (2 * (hd + 16) * U * A[:, None] + (2 * N + 16) * U) * W
+            assert torch.equal(out[t].isfinite(), finite), (i, j)
+            assert bool(((out[t].double() - want).abs() <= tol)[finite].all()), (i, j)
+            t += 1
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.float16])
+@pytest.mark.parametrize("H,KV,hd,ps", [(8, 4, 16, 16), (16, 2, 64, 16), (10, 2, 128, 32)])
+@pytest.mark.parametrize("new,prefix", [(1, 300), (20, 0), (20, 300)])
+@pytest.mark.parametrize("where", ["keys", "values", "prefix keys", "prefix values"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_is_not_finite_in_chunks_and_prefixes(value, where, new, prefix, H, KV, hd, ps, kv):
+    """One element of one kv head's keys or values, in units that all rows see whole and in others."""
+    if "prefix" in where and not prefix:
+        where = where.split()[1]
+    past = [0, 17, 140, 400]
+    c = make(len(past), H, KV, hd, ps, kv, past, [new] * len(past), seed=hd, prefix=prefix)
+    pool = c["kp" if "keys" in where else "vp"]
+    if "prefix" in where:
+        c["prefix_pages"] = c["prefix_pages"].clone()
+        pool[int(c["prefix_pages"][131 // ps]), 131 % ps, KV - 1, 5] = value
+    else:
+        for i, a in enumerate(past):
+            for at, g in ((a // 2, i % KV), (a + new - 1 - new // 3, (i + 1) % KV)):
+                pool[int(c["table"][i, at // ps]), at % ps, g, (3 * i) % hd] = value
+    check_definition(c, attend(c))

@@ -119,6 +119,54 @@ constexpr float kUnseen = -FLT_MAX;
 // A maximum to subtract: nothing seen yet counts as 0, so that the weights are 2^-inf = 0.
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+// The state of one query row over keys [key0, key1) of kv head kv in FP32, one product
+// after the other, by a warp (lane: dims lane, lane + 32, ..): for rows whose sum of weights
+// is not a number.  In the MMAs that may be the doing of the operands' parts (inf - inf),
+// of another kv head's key (times zeros) or of a key marked for its value; here a
+// score is its own, and one of -inf is a weight of 0.  Ends where nothing but NaN can follow,
+// a page out of range among it.
+template <typename KT>
+__device__ __forceinline__ void plain_row(const Batch& b, const int32_t* table, const float* q, int hd, int kv, int key0,
+                                          int key1, float scale, float& m, float& l, float (&o)[4]) {
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = 0.f;
+#pragma unroll 1
+  for (int key = key0; key < key1; ++key) {
+    const int id = __ldg(table + (key >> b.shift));
+    if ((unsigned)id >= (unsigned)b.n_pages) {
+      l = NAN;
+      return;
+    }
+    const int64_t at = id * b.page_stride + (key & ((1 << b.shift) - 1)) * b.slot_stride + kv * b.head_stride + lane;
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < hd) x = fmaf(__ldg(q + lane + 32 * e), (float)static_cast<const KT*>(b.k)[at + 32 * e], x);
+#pragma unroll
+    for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+    x *= scale;
+    const bool up = x > m;
+    const float f = up ? ex2(m - x) : 1.f;
+    if (up) m = x;
+    const float p = ex2(x - ref_of(m));
+    l = fmaf(l, f, p);
+    bool nan = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < hd) {
+        o[e] = fmaf(p, (float)static_cast<const KT*>(b.v)[at + 32 * e], o[e] * f);
+        nan = nan && o[e] != o[e];
+      }
+    if (l != l || __all_sync(0xffffffffu, nan)) {
+      l = NAN;
+      return;
+    }
+  }
+}
+
 // The pool's tensor map (paged_decode.cu).
 int32_t pool_map(const Batch& b, void* pool, int hd, int es, int F, int rows, int segments, CUtensorMap* map,
                  bool* swap);

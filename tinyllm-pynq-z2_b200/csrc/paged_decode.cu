@@ -351,39 +351,15 @@ struct Workers {
   __device__ __forceinline__ int64_t end() const { return muldiv(me + 1, units, count); }
 };
 
-// The state of a piece in FP32, one product after the other.  A page out of range leaves NaN.
+// The state of a piece by plain_row.
 template <typename KT>
-__device__ void plain_piece(const DecodeArgs& a, int s, int h0, int nr, int key0, int key1, bool whole,
-                                         float* slot) {
-  const Batch& b = a.b;
+__device__ void plain_piece(const DecodeArgs& a, int s, int h0, int nr, int key0, int key1, bool whole, float* slot) {
   const int lane = threadIdx.x & 31;
   for (int n = 0; n < nr; ++n) {
     const int h = h0 + n;
-    const float* q = a.q + s * a.ldq + (int64_t)h * a.hd;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int key = key0; key < key1; ++key) {
-      const int id = __ldg(b.table + s * b.table_stride + (key >> b.shift));
-      if ((unsigned)id >= (unsigned)b.n_pages) {
-        l = NAN;
-        break;
-      }
-      const int64_t at = id * b.page_stride + (key & ((1 << b.shift) - 1)) * b.slot_stride + h / b.rep * b.head_stride;
-      const KT* k = static_cast<const KT*>(b.k) + at;
-      const KT* v = static_cast<const KT*>(b.v) + at;
-      float x = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < a.hd) x = fmaf(__ldg(q + lane + 32 * e), (float)k[lane + 32 * e], x);
-#pragma unroll
-      for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-      x *= a.scale;
-      const float f = x > m ? ex2(m - x) : 1.f, p = ex2(x - ref_of(x > m ? x : m));
-      if (x > m) m = x;
-      l = fmaf(l, f, p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < a.hd) o[e] = fmaf(p, (float)v[lane + 32 * e], o[e] * f);
-    }
+    float m, l, o[4];
+    plain_row<KT>(a.b, a.b.table + s * a.b.table_stride, a.q + s * a.ldq + (int64_t)h * a.hd, a.hd, h / a.b.rep, key0, key1,
+                  a.scale, m, l, o);
     const int64_t row = (int64_t)s * a.H + h;
     const float inv = !whole || a.state ? 1.f : (l == 0.f ? 0.f : 1.f / l);
     float* dst = whole ? a.out + row * a.hd : slot + n * a.hd;
@@ -400,9 +376,7 @@ __device__ void plain_piece(const DecodeArgs& a, int s, int h0, int nr, int key0
 }
 
 // Goes over a warp's stretch once more and makes the pieces anew whose sum of weights
-// is not a number.  That may be another kv head's doing (its infinite key times this
-// head's zeros in the MMA) or the parts' (inf - inf); here a key's score is its own,
-// and one of -inf is a weight of 0.
+// is not a number.
 template <int HDF, typename KT>
 __device__ __noinline__ void plain_pieces(const DecodeArgs& a, const Line& line) {
   const Batch& b = a.b;

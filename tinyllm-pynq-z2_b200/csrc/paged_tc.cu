@@ -39,7 +39,8 @@
 // Load warps fetch FP16 units by TMA boxes; FP32 units, units with a bad page
 // id and units that some row does not see whole go through registers: keys no
 // row sees become zeros, and a key whose value is not finite becomes a NaN key
-// with zero values, so that only the rows that see it become NaN.
+// with zero values, so that only the rows that see it become NaN.  The softmax
+// warps make rows whose sum of weights is not a number anew at their end (plain_row).
 //
 // Blocks' units lie on one line; every CTA takes an equal stretch (as the
 // decode kernel's warps do).  Every wait is bounded; a timeout sets the status
@@ -393,6 +394,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
   __shared__ volatile int stop;
   __shared__ float row_max[S::HALVES][2][128], row_sum[S::HALVES][128];  // what a row's two threads tell one another
   __shared__ uint32_t odd_keys[4];  // keys of the unit whose values are not finite
+  __shared__ int odd[S::SOFT];      // a row of the softmax warp's has a sum of weights that is not a number
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   if (warp == S::SOFT + 4) {
@@ -417,6 +419,7 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     }
     mbar_init(&drain, 1);
     stop = 0;
+    for (int i = 0; i < S::SOFT; ++i) odd[i] = 0;
     fence_mbar_init();
   }
   tc::tc_fence_before();
@@ -444,6 +447,25 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
     return false;
   };
   auto tile_col = [&](int t) { return tmem + t * S::TC; };
+  // Where a walk's piece leaves the state of a row of its block (`orow`: the output's):
+  // the outputs' place, and that of (m, l) or null.
+  auto place = [&](const Walk<S::ROWS, KEYS>& v, int row, int64_t orow, float*& ml) {
+    const bool begin = v.p.u0 == 0;
+    if (!a.prefix && begin && v.p.u1 == v.p.units) {
+      ml = a.state ? a.state + orow * 2 : nullptr;
+      return a.out + orow * HD;
+    }
+    int64_t at;
+    if (a.prefix) {
+      // piece k of item (kv, j): the CTA's number among the item's
+      const int k = (int)(c - owner_of(v.p.x - v.p.u0, units, workers));
+      at = ((int64_t)k * a.items + (int64_t)v.p.kv * v.blocks() + v.p.j) * S::ROWS + row;
+    } else {
+      at = (c * 2 + (v.p.x == x0 && !begin ? 0 : 1)) * S::ROWS + row;
+    }
+    ml = a.part_ml + at * 2;
+    return a.part + at * HD;
+  };
   int loaded = 0;  // units that this (load) warp put into shared memory
 
   if (warp >= S::SOFT && warp < S::SOFT + 4) {
@@ -954,28 +976,13 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
         }
         tc::tc_fence_before();
       }
+      if (ok && l != l) odd[warp] = 1;
       if (in) {
         const bool begin = w.p.u0 == 0, whole = begin && w.p.u1 == w.p.units;
         const float m = ref == kUnseen ? -INFINITY : ref;
-        float* dst;
         float* ml;
-        float inv = 1.f;
-        if (a.prefix) {
-          // piece k of item (kv, j): the CTA's number among the item's
-          const int64_t first = w.p.x - w.p.u0;
-          const int k = (int)(c - owner_of(first, units, workers));
-          const int64_t at = (((int64_t)k * a.items + (int64_t)w.p.kv * w.blocks() + w.p.j) * S::ROWS + t * 128 + r);
-          dst = a.part + at * HD;
-          ml = a.part_ml + at * 2;
-        } else if (!whole) {
-          const int64_t at = (c * 2 + (w.p.x == x0 && !begin ? 0 : 1)) * S::ROWS + t * 128 + r;
-          dst = a.part + at * HD;
-          ml = a.part_ml + at * 2;
-        } else {
-          dst = a.out + (token * a.H + h) * HD;
-          ml = a.state ? a.state + (token * a.H + h) * 2 : nullptr;
-          if (!ml) inv = l == 0.f ? 0.f : 1.f / l;
-        }
+        float* dst = place(w, t * 128 + r, token * a.H + h, ml);
+        const float inv = ml ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int d = 0; d < MYD; d += 4)
           *reinterpret_cast<float4*>(dst + hf * MYD + d) =
@@ -988,6 +995,37 @@ __global__ void __launch_bounds__(TcShape<HD, KT>::THREADS, 1)
           const int64_t lastu = w.p.x - w.p.u0 + w.p.units - 1;
           a.desc[c * 2] = make_int4(w.p.tok0, w.p.kv, w.p.j, (int)(owner_of(lastu, units, workers) - c) + 1);
           a.desc[c * 2 + 1] = make_int4(w.rows(), 0, 0, 0);
+        }
+      }
+    }
+    // ---- rows whose sum of weights is not a number, anew (a warp its own, all dims)
+    ok = agree(ok);
+    __syncwarp();
+    if (ok && hf == 0 && odd[warp]) {
+      Walk<S::ROWS, KEYS> v(a);
+      v.begin(muldiv(c, units, workers), muldiv(c + 1, units, workers));
+      for (; v.more(); v.next()) {
+        const int n = v.rows() - t * 128;
+        float* ml;
+        for (int i = 0; i < 32; ++i) {
+          const int row = (warp & 3) * 32 + i, ri = v.p.j * S::ROWS + t * 128 + row;
+          if (row >= n) break;
+          const int tok = ri / a.b.rep, h = v.p.kv * a.b.rep + (ri - tok * a.b.rep);
+          float* dst = place(v, t * 128 + row, (int64_t)(v.p.tok0 + tok) * a.H + h, ml);
+          const float was = ml ? ml[1] : dst[0];
+          if (was == was) continue;
+          float m, l, o[4];
+          plain_row<KT>(a.b, a.prefix ? a.b.table : a.b.table + v.p.s * a.b.table_stride,
+                        a.q + (v.p.tok0 + tok) * a.ldq + (int64_t)h * HD, HD, v.p.kv, v.p.u0 * KEYS,
+                        min(v.p.u1 * KEYS, v.seen(tok)), a.scale, m, l, o);
+          const float inv = ml ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (lane + 32 * e < HD) dst[lane + 32 * e] = o[e] * inv;
+          if (ml && lane == 0) {
+            ml[0] = m;
+            ml[1] = l;
+          }
         }
       }
     }
