@@ -425,10 +425,11 @@ Q6W_API size_t q6w_paged_workspace_bytes(const q6w_paged_batch* batch, int32_t n
  * -- q6w_gqa_attention for one token a sequence (torch_benchmark.py:113-119),
  * and a prompt's or a chunk's attention for more.  queries (rotated)
  * [n_tokens, n_heads, head_dim] FP32 with a token stride in elements
- * (a multiple of 4); output [n_tokens, n_heads, head_dim] contiguous.
- * n_heads is a multiple of kv_heads, n_tokens * n_heads is below 2^31 - 512,
- * and page_size * head_dim elements are at least 128 bytes (append takes
- * smaller pages; head dims 256 and 512 of q6w_gqa_attention are not offered).
+ * (a multiple of 4); output [n_tokens, n_heads, head_dim] contiguous, apart
+ * from the queries.  n_heads is a multiple of kv_heads, n_tokens * n_heads is
+ * at most 2^31 - 513, and page_size * head_dim elements are at least 128 bytes
+ * (append takes smaller pages; head dims 256 and 512 of q6w_gqa_attention are
+ * not offered).
  * A token with no visible key (length 0, padding by length) gives zeros; rows
  * of tokens that no sequence holds are zeroed when zero_padding is set and
  * left as they were otherwise.  Slots behind a sequence's length, and in a

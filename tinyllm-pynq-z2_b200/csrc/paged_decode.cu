@@ -33,8 +33,8 @@
 // Layout of the work.  An item is (sequence, F kv heads, block of up to eight
 // query heads), cut into units of 16 keys (32 where rows have up to 128 bytes).  More
 // than eight heads a kv head are items of their own that read the keys again (64
-// requests of 128-8192 FP16 keys, heads of 64: 117 us with 8 a kv head, 197 with 16).  The units of all items lie on one
-// line (a prefix sum of the lengths, taken by every CTA for itself), and every
+// requests of 128-8192 FP16 keys, heads of 64: 117 us with 8 a kv head, 197 with 16).
+// The units of all items lie on one line (a prefix sum of the lengths, taken by every CTA for itself), and every
 // warp takes an equal stretch of it: ragged lengths and few long sequences
 // balance alike.  A warp that holds an item whole writes its output; pieces
 // of an item go through the workspace, joined by their CTA when it holds them

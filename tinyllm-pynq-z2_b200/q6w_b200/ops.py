@@ -405,7 +405,8 @@ def paged_attention(queries, key_pages, value_pages, page_table, lengths, query_
     other arguments as ``paged_append`` takes them, after it has run: a token
     sees its sequence's positions up to its own.  Returns [T, heads, hd];
     a token without a visible key gives zeros, and so do rows of tokens that
-    no sequence holds (in ``out``, if given, they stay as they were).
+    no sequence holds (in ``out``, if given, they stay as they were; ``out``
+    must not overlap ``queries``).
 
     Single tokens are fastest without ``query_starts``, in a call of their
     own: with it every sequence takes tiles of 128 or 256 rows (tokens times
